@@ -25,6 +25,9 @@ EXPORTS = ("ea_attention_cuda", "ea_attention_cuda_ranges", "ea_round_ratio_cuda
            "ea_kernel_timing", "ea_attention_cuda_paged", "ea_kv_append_cuda", "ea_selftest_fast64",
            "ea_merge_partials_nccl", "ea_set_test_hooks", "ea_last_host_stats",
            "ea_partials_merge_gathered_cuda")
+# ... and include/exactattn_serving.h
+SERVING_EXPORTS = ("ea_plan_step_cuda", "ea_rope_cuda", "ea_tree_attention_workspace", "ea_tree_attention_cuda",
+                   "ea_process_logits_cuda", "ea_serving_last_error")
 WIDE_DIGITS = 48  # EA_WIDE_DIGITS
 
 
@@ -72,6 +75,46 @@ class KvAppendArgs(ctypes.Structure):
                 ("k_meta", ctypes.c_void_p), ("batch", ctypes.c_int64), ("kv_heads", ctypes.c_int),
                 ("page_size", ctypes.c_int), ("max_pages", ctypes.c_int), ("n_new", ctypes.c_int),
                 ("d", ctypes.c_int), ("advance_lens", ctypes.c_int)]
+
+
+def _fields(spec: str):
+    """ctypes fields of "type: name name; ..." (p pointer, l int64, i int, f float)."""
+    kinds = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float}
+    return [(name, kinds[kind.strip()]) for part in spec.split(";") if part.strip()
+            for kind, names in [part.split(":")] for name in names.split()]
+
+
+class PlanStepArgs(ctypes.Structure):
+    """ea_plan_step_t (include/exactattn_serving.h), field for field."""
+    _fields_ = _fields("p: context_lens new_lens page_table free_pages free_head depths slot_map positions token_seq "
+                       "q_start seq_lens next_free_head status; l: table_stride; "
+                       "i: batch max_pages page_size num_free max_tokens")
+
+
+class RopeArgs(ctypes.Structure):
+    """ea_rope_t (include/exactattn_serving.h)."""
+    _fields_ = _fields("p: q k v; l: q_stride k_stride v_stride q_head_stride k_head_stride v_head_stride; "
+                       "p: positions; l: axis_stride; p: inv_freq axes q_out k_out slot_map k_cache v_cache; "
+                       "l: k_page_stride k_cache_head_stride k_row_stride v_page_stride v_cache_head_stride "
+                       "v_row_stride tokens num_slots; "
+                       "i: q_heads kv_heads d rot num_axes page_size dtype adjacent inverse")
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """ea_tree_attention_t (include/exactattn_serving.h)."""
+    _fields_ = _fields("p: q; l: q_stride q_head_stride; p: k_cache v_cache; "
+                       "l: k_page_stride k_head_stride k_row_stride v_page_stride v_head_stride v_row_stride; "
+                       "p: page_table; l: table_stride; p: seq_lens q_start tree_mask out lse workspace; "
+                       "l: tokens num_pages; f: alpha; "
+                       "i: batch q_heads kv_heads d page_size max_pages mask_words max_new dtype")
+
+
+class ProcessLogitsArgs(ctypes.Structure):
+    """ea_process_logits_t (include/exactattn_serving.h)."""
+    _fields_ = _fields("p: logits out; l: logits_stride out_stride; p: row_seq history; l: history_stride; "
+                       "p: history_lens prompt_lens repetition frequency presence bias_ids bias_values allowed_bits; "
+                       "l: mask_stride; p: mask_rows draft_tokens q_start tree_mask; l: rows; "
+                       "i: vocab batch max_history num_biases num_masks tree_words dtype")
 
 
 def load(path: str | None = None):
@@ -139,6 +182,14 @@ def load(path: str | None = None):
     lib.ea_cuda_release.restype = None
     lib.ea_cuda_last_error.argtypes = []
     lib.ea_cuda_last_error.restype = ctypes.c_char_p
+    for name, args in (("ea_plan_step_cuda", PlanStepArgs), ("ea_rope_cuda", RopeArgs),
+                       ("ea_tree_attention_cuda", TreeAttentionArgs), ("ea_process_logits_cuda", ProcessLogitsArgs)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), P]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.ea_tree_attention_workspace.argtypes = [ctypes.POINTER(TreeAttentionArgs)]
+    lib.ea_tree_attention_workspace.restype = ctypes.c_int64
+    lib.ea_serving_last_error.argtypes = []
+    lib.ea_serving_last_error.restype = ctypes.c_char_p
     if path is None:
         _lib = lib
     return lib

@@ -16,13 +16,13 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "libexactattn_cuda.so")
 SOURCES = ["ea_simt.cu", "ea_tc.cu", "ea_decode.cu", "ea_api.cu", "ea_synth.cu", "ea_noalloc.cu", "ea_cache.cu",
-           "ea_selftest.cu", "ea_nccl.cu"]
+           "ea_selftest.cu", "ea_nccl.cu", "ea_plan.cu", "ea_rope.cu", "ea_tree.cu", "ea_logits.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
-HEADER = os.path.join(HERE, "..", "include", "exactattn_cuda.h")
+HEADERS = [os.path.join(HERE, "..", "include", f) for f in ("exactattn_cuda.h", "exactattn_serving.h")]
 
 
 def _headers_mtime() -> float:
-    hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))] + [HEADER]
+    hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))] + HEADERS
     return max(os.path.getmtime(p) for p in hs if os.path.exists(p))
 
 

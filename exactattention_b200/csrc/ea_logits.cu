@@ -1,0 +1,227 @@
+// Penalties for repeated tokens, biases and grammar masks on logits (ea_process_logits_cuda).
+//
+// Bound by HBM: a row's logits are read once and written once. A block owns a chunk of one row's
+// vocabulary. What changes a token beyond its mask bit is kept in a table of one 32-bit word per token
+// of the chunk in shared memory, built from the row's history, path and bias list:
+//   bits 0-19 how often the token was generated, bits 20-30 which bias entry it has first
+//   (EA_LOGITS_MAX_BIASES - entry, 0: none), bit 31 whether the prompt holds it.
+// The words are integers, so the order of the atomics cannot change them. The first logits are loaded
+// before the table is built, so their latency overlaps the scan of the history. Rows without penalties
+// and biases build no table.
+#include "ea_serving.cuh"
+
+namespace ea {
+namespace serving {
+namespace {
+
+constexpr int THREADS = 512;
+constexpr int UNROLL = 4;  // 16-byte pieces a thread has in flight
+constexpr uint32_t COUNT = 0xFFFFFu, PROMPT = 0x80000000u;
+constexpr int CODE_SHIFT = 20;
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+struct Row {
+  float rep, freq, pres;
+  const int32_t* ids;
+  const float* vals;
+  bool dup;
+};
+
+// The row's rule for one token whose table word is not zero.
+__device__ __noinline__ float adjust(float x, uint32_t w, int token, const Row& r, int num_biases) {
+  const uint32_t cnt = w & COUNT, code = (w >> CODE_SHIFT) & 0x7FFu;
+  if (cnt || (w & PROMPT)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
+  x = __fsub_rn(x, __fmul_rn(r.freq, (float)cnt));
+  if (cnt) x = __fsub_rn(x, r.pres);
+  if (code) {
+    int e = EA_LOGITS_MAX_BIASES - (int)code;
+    x = __fadd_rn(x, r.vals[e]);
+    if (r.dup)
+      for (++e; e < num_biases; ++e)
+        if (r.ids[e] == token) x = __fadd_rn(x, r.vals[e]);
+  }
+  return x;
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(THREADS) logits_kernel(ea_process_logits_t a, int chunk, FastDiv by_chunks,
+                                                         int chunks) {
+  using P = Pack<T, VEC>;
+  extern __shared__ uint4 table4[];
+  uint32_t* table = (uint32_t*)table4;
+  __shared__ int dup;
+  const int tid = threadIdx.x;
+  const int64_t row = div_by(blockIdx.x, by_chunks);
+  const int part = (int)(blockIdx.x - row * chunks);
+  const T* src = (const T*)a.logits + row * a.logits_stride;
+  T* dst = (T*)a.out + row * a.out_stride;
+  // Pieces are aligned in memory: place i of the chunk is token v0 + i, and the row's first piece may
+  // begin before its first token.
+  const int mis = (int)(((uintptr_t)src / sizeof(T)) % VEC);
+  const int v0 = part * chunk - mis;
+  if (v0 >= a.vocab) return;
+
+  P x[UNROLL];
+#pragma unroll
+  for (int j = 0; j < UNROLL; ++j) {
+    const int i = (j * THREADS + tid) * VEC, v = v0 + i;
+    if (i < chunk && v >= 0 && v + VEC <= a.vocab) x[j] = *(const P*)(src + v);
+  }
+
+  const int b = a.row_seq ? a.row_seq[row] : (int)row;
+  const bool real = b >= 0 && b < a.batch;
+  const int m = a.allowed_bits && real ? (a.mask_rows ? a.mask_rows[row] : (int)row) : -1;
+  const uint32_t* bits = m >= 0 && m < a.num_masks ? (const uint32_t*)a.allowed_bits + m * a.mask_stride : nullptr;
+  Row r;
+  r.rep = real && a.repetition ? a.repetition[b] : 1.0f;
+  r.freq = real && a.frequency ? a.frequency[b] : 0.0f;
+  r.pres = real && a.presence ? a.presence[b] : 0.0f;
+  r.ids = a.bias_ids + (int64_t)(real ? b : 0) * a.num_biases;
+  r.vals = a.bias_values + (int64_t)(real ? b : 0) * a.num_biases;
+  r.dup = false;
+  const bool counts = real && (r.rep != 1.0f || r.freq != 0.0f || r.pres != 0.0f) && (a.history || a.draft_tokens);
+  const bool biased = real && a.num_biases > 0;
+  const bool tabled = counts || biased;
+  if (tabled) {
+    for (int i = tid; i < chunk / 4; i += THREADS) table4[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) dup = 0;
+    __syncthreads();
+    const uint32_t lo = (uint32_t)max(v0, 0), span = (uint32_t)(min(a.vocab, v0 + chunk)) - lo;
+    uint32_t* at = table + ((int)lo - v0);
+    if (counts && a.history) {
+      const int n = min(max(a.history_lens[b], 0), a.max_history);
+      const int np = a.prompt_lens ? min(max(a.prompt_lens[b], 0), n) : 0;
+      const int32_t* h = a.history + (int64_t)b * a.history_stride;
+      for (int i = tid; i < n; i += THREADS) {
+        const uint32_t t = (uint32_t)h[i] - lo;
+        if (t < span) {
+          if (i < np) atomicOr(at + t, PROMPT);
+          else atomicAdd(at + t, 1u);
+        }
+      }
+    }
+    if (counts && a.draft_tokens) {
+      const int64_t q0 = a.q_start[b], q1 = min((int64_t)a.q_start[b + 1], a.rows);
+      if (q0 >= 0 && q0 < q1) {
+        const int n = (int)min(q1 - q0, (int64_t)(a.tree_mask ? a.tree_words * 32 : row - q0 + 1));
+        for (int j = tid; j < min(n, EA_LOGITS_MAX_PATH); j += THREADS) {
+          if (a.tree_mask && !((a.tree_mask[row * a.tree_words + (j >> 5)] >> (j & 31)) & 1)) continue;
+          const uint32_t t = (uint32_t)a.draft_tokens[q0 + j] - lo;
+          if (t < span) atomicAdd(at + t, 1u);
+        }
+      }
+    }
+    if (biased) {
+      __syncthreads();
+      for (int e = tid; e < a.num_biases; e += THREADS) {
+        const uint32_t t = (uint32_t)r.ids[e] - lo;
+        if (t < span) {
+          const uint32_t code = (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT;
+          const uint32_t old = atomicMax(at + t, (at[t] & (PROMPT | COUNT)) | code);
+          if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
+        }
+      }
+    }
+    __syncthreads();
+    r.dup = dup != 0;
+  }
+
+  for (int i0 = 0; i0 < chunk; i0 += UNROLL * THREADS * VEC) {
+    if (i0) {
+#pragma unroll
+      for (int j = 0; j < UNROLL; ++j) {
+        const int i = i0 + (j * THREADS + tid) * VEC, v = v0 + i;
+        if (i < chunk && v >= 0 && v + VEC <= a.vocab) x[j] = *(const P*)(src + v);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      const int i = i0 + (j * THREADS + tid) * VEC, v = v0 + i;
+      if (i >= chunk || v >= a.vocab || v + VEC <= 0) continue;
+      const bool whole = v >= 0 && v + VEC <= a.vocab;
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (v + e >= 0 && v + e < a.vocab) x[j].v[e] = src[v + e];
+      }
+      if (tabled) {
+        uint32_t w[VEC], any = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] = table[i + e], any |= w[e];
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (w[e]) x[j].v[e] = from_f<T>(adjust(to_f(x[j].v[e]), w[e], v + e, r, a.num_biases));
+        }
+      }
+      if (bits) {
+        // bit e: token v + e is allowed; the piece may lie in two words
+        const int first = max(v, 0), last = min(v + VEC, a.vocab) - 1;
+        const uint32_t w0 = bits[first >> 5], w1 = bits[last >> 5];
+        const uint32_t ok = __funnelshift_r(w0, w1, first & 31);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (v + e >= first && v + e <= last && !((ok >> (v + e - first)) & 1)) x[j].v[e] = from_f<T>(-INFINITY);
+      }
+      if (whole) {
+        *(P*)(dst + v) = x[j];
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (v + e >= 0 && v + e < a.vocab) dst[v + e] = x[j].v[e];
+      }
+    }
+  }
+}
+
+template <typename T, int VEC>
+int launch(const ea_process_logits_t& a, cudaStream_t st) {
+  // The largest chunk whose blocks still fill the GPU twice: fewer chunks read the history less often.
+  int chunk = 16384;
+  while (chunk > 2048 && a.rows * ((a.vocab + chunk - 1) / chunk) < 2 * sm_count()) chunk >>= 1;
+  const int chunks = (int)(((int64_t)a.vocab + VEC - 1 + chunk - 1) / chunk);
+  const int64_t blocks = a.rows * chunks;
+  if (blocks > 0x7FFFFFFF) return fail(-1, "process_logits: too many rows");
+  const size_t smem = (size_t)chunk * 4;
+  const cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+  if (e != cudaSuccess) return cuda_rc(e);
+  logits_kernel<T, VEC><<<(unsigned)blocks, THREADS, smem, st>>>(a, chunk, fast_div((uint32_t)chunks), chunks);
+  return cuda_rc(cudaGetLastError());
+}
+
+template <typename T>
+int launch_type(const ea_process_logits_t& a, cudaStream_t st) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  // 16-byte pieces where input and output rows are equally far from a 16-byte boundary
+  const bool same = ((uintptr_t)a.logits - (uintptr_t)a.out) % 16 == 0 &&
+                    (a.rows <= 1 || (a.logits_stride - a.out_stride) % VEC == 0);
+  return same ? launch<T, VEC>(a, st) : launch<T, 1>(a, st);
+}
+
+}  // namespace
+}  // namespace serving
+}  // namespace ea
+
+extern "C" int ea_process_logits_cuda(const ea_process_logits_t* a, void* stream) {
+  using namespace ea::serving;
+  if (!a || a->rows < 0 || a->vocab < 0 || a->batch < 0 || a->max_history < 0 || a->num_biases < 0 || a->num_masks < 0 ||
+      a->tree_words < 0)
+    return fail(-1, "process_logits: negative size");
+  if (a->max_history > EA_LOGITS_MAX_HISTORY || a->num_biases > EA_LOGITS_MAX_BIASES || a->vocab > (1 << 30))
+    return fail(-1, "process_logits: history, biases or vocabulary above their limits");
+  if (a->rows == 0 || a->vocab == 0) return 0;
+  if (!a->logits || !a->out || (a->history && !a->history_lens) || (a->num_biases && (!a->bias_ids || !a->bias_values)) ||
+      (a->draft_tokens && !a->q_start))
+    return fail(-1, "process_logits: a required pointer is NULL");
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (a->dtype) {
+    case EA_BF16: return launch_type<__nv_bfloat16>(*a, st);
+    case EA_FP16: return launch_type<__half>(*a, st);
+    case EA_FP32: return launch_type<float>(*a, st);
+  }
+  return fail(-9, "process_logits: unknown element type");
+}

@@ -1,0 +1,470 @@
+// Attention of a step's tokens over the paged cache (ea_tree_attention_cuda): the entry, and the kernel for
+// few query rows per kv head.
+//
+// Row statistics (maximum, sum) and outputs are binary32. The kernel below keeps 16 query rows of one
+// sequence and kv head (tokens x the heads of a group) in registers as the A operand of 16 x 8 x 16 matrix
+// instructions; a warp owns 16 of a tile's 64 keys with a running maximum, sum and output of its own, so the
+// warps of a block stream their keys without waiting for one another and join once per item. Bound by HBM:
+// a 16-key slice is 8 KB of K and V at d = 128, for which an SM has about 350 cycles at the
+// measured copy rate, and needs 48 matrix instructions and 16 ldmatrix of its four sub-partitions.
+// Weights enter P.V as a pair of 16-bit numbers, their rounding and its remainder (relative
+// error 2^-17 for bf16 instead of 2^-9), which costs 16 more matrix instructions a slice: the tensor pipe
+// has the room.
+#include <type_traits>
+
+#include "ea_tree.cuh"
+
+namespace ea {
+namespace serving {
+namespace tree {
+
+namespace {
+
+constexpr int ROWS = 16, WARPS = 4, KT = 16 * WARPS, THREADS = 32 * WARPS, STAGES = 3;
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes, or zeros where `ok` is false
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack(__nv_bfloat16 x, __nv_bfloat16 y) {
+  return (uint32_t)__bfloat16_as_ushort(x) | (uint32_t)__bfloat16_as_ushort(y) << 16;
+}
+__device__ __forceinline__ uint32_t pack(__half x, __half y) {
+  return (uint32_t)__half_as_ushort(x) | (uint32_t)__half_as_ushort(y) << 16;
+}
+// two weights as their roundings and the roundings of what is left
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const T hx = from_f<T>(x), hy = from_f<T>(y);
+  hi = pack(hx, hy);
+  lo = pack(from_f<T>(x - to_f(hx)), from_f<T>(y - to_f(hy)));
+}
+// the two 16-bit numbers with infinities and NaN replaced by zeros
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t v) {
+  constexpr uint32_t EXP = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  if ((v & EXP) == EXP) v &= 0xFFFF0000u;
+  if ((v & EXP << 16) == EXP << 16) v &= 0xFFFFu;
+  return v;
+}
+// whether four pairs of numbers hold an infinity or NaN: x * 0 summed up is 0 unless one does
+template <typename T>
+__device__ __forceinline__ bool not_finite(const uint32_t* f) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const uint32_t zero = 0;
+  T2 z = *(const T2*)&zero;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z = __hfma2(*(const T2*)&f[e], *(const T2*)&zero, z);
+  return (*(const uint32_t*)&z & 0x7FFF7FFFu) != 0;
+}
+
+template <int DP>
+struct Smem {
+  static constexpr int ROW_BYTES = DP * 2;
+  static constexpr int SLICE = 16 * ROW_BYTES;                    // K or V of 16 keys
+  static constexpr int STAGE = 2 * SLICE;                         // one warp's
+  static constexpr int POOL = WARPS * STAGES * STAGE;             // also the join's scratch
+  static_assert(POOL >= WARPS * ROWS * DP * 4, "the join fits into the stages");
+};
+
+template <int DP>
+__device__ __forceinline__ uint32_t swz(int row, int piece) {
+  return (uint32_t)(row * Smem<DP>::ROW_BYTES + ((piece ^ (row & 7)) << 4));
+}
+
+// Issues the copies of 16 keys from `key0` of the item into a stage. `page` is this lane's page of key
+// key0 + lane % 16 (-1: none).
+template <typename T, int DP>
+__device__ __forceinline__ void load_slice(const Args& a, const Item& it, int key0, int page, uint32_t stage, int lane) {
+  constexpr int PIECES = DP / 8, LANES_PER_ROW = PIECES < 8 ? PIECES : 8, RPI = 32 / LANES_PER_ROW;
+  const int sub = lane / LANES_PER_ROW, c0 = lane % LANES_PER_ROW;
+#pragma unroll
+  for (int r0 = 0; r0 < 16; r0 += RPI) {
+    const int r = r0 + sub, key = key0 + r;
+    const int pg = __shfl_sync(0xffffffffu, page, r);
+    const bool ok = key < it.len && pg >= 0;
+    const int64_t off = ok ? key - (int64_t)div_by((uint32_t)key, a.by_page) * a.t.page_size : 0;
+    const int64_t p = ok ? pg : 0;
+    const T* ks = (const T*)a.t.k_cache + p * a.t.k_page_stride + it.h * a.t.k_head_stride + off * a.t.k_row_stride;
+    const T* vs = (const T*)a.t.v_cache + p * a.t.v_page_stride + it.h * a.t.v_head_stride + off * a.t.v_row_stride;
+#pragma unroll
+    for (int c = c0; c < PIECES; c += LANES_PER_ROW) {
+      const bool in = ok && c * 8 < a.t.d;
+      cp16(stage + swz<DP>(r, c), in ? ks + c * 8 : (const T*)a.t.k_cache, in);
+      cp16(stage + Smem<DP>::SLICE + swz<DP>(r, c), in ? vs + c * 8 : (const T*)a.t.v_cache, in);
+    }
+  }
+}
+
+__device__ __forceinline__ int page_of(const Args& a, const Item& it, int key0, int lane) {
+  const int key = key0 + (lane & 15);
+  if (key >= it.len) return -1;
+  const int p = a.t.page_table[it.b * a.t.table_stride + div_by((uint32_t)key, a.by_page)];
+  return p >= 0 && p < a.t.num_pages ? p : -1;
+}
+
+// Whether query row R of the item (token i of the step) sees key `key`.
+__device__ __forceinline__ bool sees(const Args& a, const Item& it, int i, int key, int page_ok) {
+  if (key >= it.len || !page_ok) return false;
+  const int ctx = it.len - it.new_tokens;
+  if (key < ctx) return true;
+  const int j = key - ctx;
+  if (!a.t.tree_mask) return j <= i;
+  return (j >> 5) < a.t.mask_words && ((a.t.tree_mask[(int64_t)(it.q0 + i) * a.t.mask_words + (j >> 5)] >> (j & 31)) & 1);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
+  using S = Smem<DP>;
+  extern __shared__ __align__(128) uint8_t pool[];
+  uint32_t* sums = (uint32_t*)(pool + S::POOL);
+  __shared__ uint64_t scratch[32];
+  __shared__ float join_m[WARPS][ROWS], join_l[WARPS][ROWS];
+  __shared__ float weights[WARPS][ROWS][17];  // the slow path's weights, -1: not seen
+  Schedule<ROWS, KT> sch;
+  sch.build(a, sums, scratch);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t base = smem_addr(pool) + warp * STAGES * S::STAGE;
+  uint32_t pos = sch.share(blockIdx.x);
+  const uint32_t end = sch.share(blockIdx.x + 1);
+  const float alpha = a.t.alpha;
+
+  while (pos < end) {
+    const Item it = sch.item(a, pos, end);
+    pos += it.kt1 - it.kt0;
+    const int ctx = it.len - it.new_tokens;
+    const int rows = min(ROWS, it.new_tokens * a.group - it.m * ROWS);
+    const int R0 = it.m * ROWS;
+
+    // Q as A fragments: rows lane / 4 and lane / 4 + 8
+    uint32_t qf[DP / 16][4];
+    int tok[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = lane / 4 + 8 * half, R = R0 + min(r, rows - 1);
+      tok[half] = (int)div_by((uint32_t)R, a.by_group);
+      const int j = R - tok[half] * a.group;
+      const T* q = (const T*)a.t.q + (int64_t)(it.q0 + tok[half]) * a.t.q_stride +
+                   (int64_t)(it.h * a.group + j) * a.t.q_head_stride;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int c = ks * 16 + p * 8 + (lane & 3) * 2;
+          qf[ks][half + 2 * p] = c < a.t.d ? *(const uint32_t*)(q + c) : 0u;
+        }
+    }
+    float o[DP / 8][4];
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    const int n = it.kt1 - it.kt0;
+    const int key_w = it.kt0 * KT + warp * 16;
+    // pages one slice ahead of their copies
+    int page = page_of(a, it, key_w, lane);
+    uint32_t seen_pages[STAGES];  // which keys of a stage's slice have a page
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+      if (s < n) load_slice<T, DP>(a, it, key_w + s * KT, page, base + s * S::STAGE, lane);
+      seen_pages[s] = __ballot_sync(0xffffffffu, page >= 0);
+      cp_commit();
+      page = page_of(a, it, key_w + (s + 1) * KT, lane);
+    }
+    seen_pages[STAGES - 1] = 0;
+    int stage = 0;
+    for (int t = 0; t < n; ++t) {
+      cp_wait<STAGES - 2>();
+      __syncwarp();
+      {
+        const int nt = t + STAGES - 1;
+        int ns = stage + STAGES - 1;
+        if (ns >= STAGES) ns -= STAGES;
+        if (nt < n) load_slice<T, DP>(a, it, key_w + nt * KT, page, base + ns * S::STAGE, lane);
+        const uint32_t bl = __ballot_sync(0xffffffffu, page >= 0);
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s)
+          if (s == ns) seen_pages[s] = bl;
+        cp_commit();
+        page = page_of(a, it, key_w + (nt + 1) * KT, lane);
+      }
+      uint32_t okm = 0;
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s)
+        if (s == stage) okm = seen_pages[s];
+      const uint32_t kb = base + stage * S::STAGE, vb = kb + S::SLICE;
+      const int key0 = key_w + t * KT;
+
+      // scores: s[nt][..] rows lane / 4 (+ 8), keys nt * 8 + 2 (lane % 4) (+ 1)
+      float s[2][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        if (ks * 16 < a.t.d) {
+          uint32_t f[4];
+          ldsm4(kb + swz<DP>((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), f);
+          mma<T>(s[0], qf[ks], f[0], f[1]);
+          mma<T>(s[1], qf[ks], f[2], f[3]);
+        }
+      }
+      const bool masked = key0 + 16 > ctx || (okm & 0xFFFFu) != 0xFFFFu;
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[nt][e] *= alpha;
+          if (masked) {
+            const int kk = nt * 8 + 2 * (lane & 3) + (e & 1);
+            if (!sees(a, it, tok[e >> 1], key0 + kk, (okm >> kk) & 1)) s[nt][e] = -INFINITY;
+          }
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[nt][e]);
+        }
+      float scale[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
+        mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
+        const float mn = fmaxf(m[half], mx[half]);
+        const float ref = mn == -INFINITY ? 0.0f : mn;
+        scale[half] = exp2f(m[half] - ref);
+        m[half] = mn;
+        l[half] *= scale[half];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            s[nt][2 * half + e] = exp2f(s[nt][2 * half + e] - ref);
+            l[half] += s[nt][2 * half + e];
+          }
+      }
+      if (__any_sync(0xffffffffu, scale[0] != 1.0f || scale[1] != 1.0f)) {
+#pragma unroll
+        for (int nn = 0; nn < DP / 8; ++nn)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nn][e] *= scale[e >> 1];
+      }
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          split2<T>(s[nt][2 * half], s[nt][2 * half + 1], hi[nt * 2 + half], lo[nt * 2 + half]);
+      // an infinity or NaN among the values may not meet the zero weight of a row that does not see its key,
+      // nor a weight's remainder: such values leave the product and reach the rows that see them one by one
+      bool bad = false;
+#pragma unroll
+      for (int nn = 0; nn < DP / 16; ++nn) {
+        if (nn * 16 < a.t.d) {
+          uint32_t f[4];
+          ldsm4_t(vb + swz<DP>(lane & 15, nn * 2 + (lane >> 4)), f);
+          if (not_finite<T>(f)) {
+            bad = true;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = finite2<T>(f[e]);
+          }
+          mma<T>(o[2 * nn], hi, f[0], f[1]);
+          mma<T>(o[2 * nn + 1], hi, f[2], f[3]);
+          mma<T>(o[2 * nn], lo, f[0], f[1]);
+          mma<T>(o[2 * nn + 1], lo, f[2], f[3]);
+        }
+      }
+      if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int kk = nt * 8 + 2 * (lane & 3) + (e & 1);
+            weights[warp][lane / 4 + 8 * (e >> 1)][kk] =
+                sees(a, it, tok[e >> 1], key0 + kk, (okm >> kk) & 1) ? s[nt][e] : -1.0f;
+          }
+        __syncwarp();
+        for (int kk = 0; kk < 16; ++kk) {
+#pragma unroll
+          for (int nn = 0; nn < DP / 8; ++nn)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = nn * 8 + 2 * (lane & 3) + e;
+              const T v = *(const T*)(pool + (vb - smem_addr(pool)) + swz<DP>(kk, c >> 3) + (c & 7) * 2);
+              const float f = to_f(v);
+              if (isfinite(f)) continue;
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const float w = weights[warp][lane / 4 + 8 * half][kk];
+                if (w != -1.0f) o[nn][2 * half + e] += w * f;
+              }
+            }
+        }
+        __syncwarp();
+      }
+      if (++stage == STAGES) stage = 0;
+    }
+    cp_wait<0>();
+
+    // join the warps
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+      if ((lane & 3) == 0) join_m[warp][lane / 4 + 8 * half] = m[half], join_l[warp][lane / 4 + 8 * half] = l[half];
+    }
+    __syncthreads();  // every warp's copies have landed and its stages are free
+    float* acc = (float*)pool + warp * ROWS * DP;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = lane / 4 + 8 * half;
+      if (r < rows) {
+        float mm = join_m[0][r];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, join_m[w][r]);
+        const float sc = exp2f(m[half] - (mm == -INFINITY ? 0.0f : mm));
+#pragma unroll
+        for (int nn = 0; nn < DP / 8; ++nn)
+          *(float2*)(acc + r * DP + nn * 8 + 2 * (lane & 3)) = make_float2(o[nn][2 * half] * sc, o[nn][2 * half + 1] * sc);
+      }
+    }
+    __syncthreads();
+    const bool whole = it.kt0 == 0 && it.kt1 == it.tiles;
+    float* slot = slot_of(a, 2 * blockIdx.x + (it.kt0 == 0 ? 1 : 0), ROWS);
+    for (int e = tid; e < rows * DP; e += THREADS) {
+      const int r = e / DP, c = e % DP;
+      float mm = join_m[0][r], ll = 0.0f, x = 0.0f;
+#pragma unroll
+      for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, join_m[w][r]);
+      const float ref = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        ll = fmaf(join_l[w][r], exp2f(join_m[w][r] - ref), ll);
+        x += ((const float*)pool)[(w * ROWS + r) * DP + c];
+      }
+      if (whole) {
+        const int R = R0 + r, i = (int)div_by((uint32_t)R, a.by_group), j = R - i * a.group;
+        const int64_t head = (int64_t)(it.q0 + i) * a.t.q_heads + it.h * a.group + j;
+        if (c < a.t.d) ((T*)a.t.out)[head * a.t.d + c] = from_f<T>(ll == 0.0f ? 0.0f : x / ll);
+        if (c == 0 && a.t.lse) a.t.lse[head] = ll == 0.0f ? -INFINITY : mm + log2f(ll);
+      } else {
+        slot[r * DP + c] = x;
+        if (c == 0) slot[ROWS * DP + r] = mm, slot[ROWS * (DP + 1) + r] = ll;
+      }
+    }
+    __syncthreads();  // before the next item's copies
+  }
+}
+
+template <typename T, int DP>
+int launch(Args& a, cudaStream_t st) {
+  const size_t smem = Smem<DP>::POOL + 4 * (size_t)(a.t.batch + 1);
+  const size_t csmem = 4 * (size_t)(a.t.batch + 1);
+  cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return cuda_rc(e);
+  few_rows_kernel<T, DP><<<a.workers, THREADS, smem, st>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_rc(e);
+  if (a.workers > 1) combine_kernel<T, ROWS, KT, 256><<<a.workers, 256, csmem, st>>>(a);
+  return cuda_rc(cudaGetLastError());
+}
+
+// Most units a call can have, from the sizes the host knows.
+int64_t most_units(const ea_tree_attention_t& t, int rows, int kt) {
+  const int64_t group = t.q_heads / t.kv_heads;
+  const int64_t tiles = ((int64_t)t.max_pages * t.page_size + kt - 1) / kt;
+  // row tiles: every sequence's last one may be partly filled
+  const int64_t row_tiles = t.tokens * group / rows + t.batch;
+  return row_tiles * t.kv_heads * (tiles > 0 ? tiles : 1);
+}
+
+int check(const ea_tree_attention_t* t) {
+  if (!t || t->tokens < 0 || t->batch < 0 || t->q_heads <= 0 || t->kv_heads <= 0 || t->d <= 0 || t->page_size <= 0 ||
+      t->max_pages < 0 || t->num_pages < 0 || t->mask_words < 0)
+    return fail(-1, "tree_attention: negative or zero size");
+  if (t->q_heads % t->kv_heads) return fail(-1, "tree_attention: q_heads is no multiple of kv_heads");
+  if (t->batch > EA_TREE_MAX_SEQS) return fail(-1, "tree_attention: more than EA_TREE_MAX_SEQS sequences");
+  if (t->d % 8 || t->d > 128) return fail(-9, "tree_attention: d is no multiple of 8 up to 128");
+  if (t->dtype != EA_BF16 && t->dtype != EA_FP16) return fail(-9, "tree_attention: element type is neither bf16 nor fp16");
+  if (t->tokens * t->q_heads >= (1ll << 31) || (int64_t)t->max_pages * t->page_size >= (1ll << 31) ||
+      most_units(*t, ROWS, KT) >= (1ll << 31))
+    return fail(-1, "tree_attention: too many tokens or keys");
+  return 0;
+}
+
+int workers_for(const ea_tree_attention_t& t) {
+  const int64_t most = most_units(t, ROWS, KT), fill = 2 * (int64_t)sm_count();
+  return (int)(most < fill ? (most > 0 ? most : 1) : fill);
+}
+
+}  // namespace
+}  // namespace tree
+}  // namespace serving
+}  // namespace ea
+
+extern "C" int64_t ea_tree_attention_workspace(const ea_tree_attention_t* t) {
+  using namespace ea::serving;
+  if (tree::check(t)) return -1;
+  const int dp = t->d <= 64 ? 64 : 128;
+  return (int64_t)tree::workers_for(*t) * 2 * tree::ROWS * (dp + 2) * 4;
+}
+
+extern "C" int ea_tree_attention_cuda(const ea_tree_attention_t* t, void* stream) {
+  using namespace ea::serving;
+  const int rc = tree::check(t);
+  if (rc) return rc;
+  if (t->tokens == 0 || t->batch == 0) return 0;
+  if (!t->q || !t->out || !t->q_start || !t->seq_lens || !t->workspace ||
+      (t->max_pages && (!t->page_table || !t->k_cache || !t->v_cache)))
+    return fail(-1, "tree_attention: a required pointer is NULL");
+  const uintptr_t base = (uintptr_t)t->q | (uintptr_t)t->k_cache | (uintptr_t)t->v_cache | (uintptr_t)t->workspace;
+  const int64_t strides = t->q_stride | t->q_head_stride | t->k_page_stride | t->k_head_stride | t->k_row_stride |
+                          t->v_page_stride | t->v_head_stride | t->v_row_stride;
+  if (base % 16 || strides % 8) return fail(-9, "tree_attention: rows are not on 16-byte boundaries");
+  tree::Args a;
+  a.t = *t;
+  a.group = t->q_heads / t->kv_heads;
+  a.by_page = fast_div((uint32_t)t->page_size);
+  a.by_group = fast_div((uint32_t)a.group);
+  a.dp = t->d <= 64 ? 64 : 128;
+  a.workers = tree::workers_for(*t);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (t->dtype == EA_BF16)
+    return a.dp == 64 ? tree::launch<__nv_bfloat16, 64>(a, st) : tree::launch<__nv_bfloat16, 128>(a, st);
+  return a.dp == 64 ? tree::launch<__half, 64>(a, st) : tree::launch<__half, 128>(a, st);
+}
