@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -36,6 +37,7 @@ def needs_build() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         build_synth_host()
+        build_serving_native()
         return OUT
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     os.makedirs(OBJ, exist_ok=True)
@@ -57,6 +59,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
                     "-o", tmp, *objs], check=True)
     os.replace(tmp, OUT)
     build_synth_host(force)
+    build_serving_native(force)
     return OUT
 
 
@@ -70,6 +73,27 @@ def build_synth_host(force: bool = False) -> str:
         subprocess.run(["gcc", "-O3", "-fopenmp", "-fPIC", "-shared", "-o", SYNTH_HOST + ".tmp", src], check=True)
         os.replace(SYNTH_HOST + ".tmp", SYNTH_HOST)
     return SYNTH_HOST
+
+
+SERVING_NATIVE = os.path.join(HERE, "_serving_native" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_serving_native(force: bool = False) -> str:
+    """The Python binding of the serving operators (csrc/ea_serving_py.cpp), g++ against torch's headers; it
+    finds libexactattn_cuda.so beside itself."""
+    src = os.path.join(CSRC, "ea_serving_py.cpp")
+    deps = [src, HEADERS[1]]
+    if force or not os.path.exists(SERVING_NATIVE) or os.path.getmtime(SERVING_NATIVE) < max(map(os.path.getmtime, deps)):
+        from torch.utils import cpp_extension
+
+        cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))
+        inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+        lib = cpp_extension.library_paths()
+        subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-I{p}" for p in inc], "-o", SERVING_NATIVE + ".tmp",
+                        src, *[f"-L{p}" for p in lib], f"-L{HERE}", "-l:libexactattn_cuda.so", "-lc10", "-lc10_cuda",
+                        "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], check=True)
+        os.replace(SERVING_NATIVE + ".tmp", SERVING_NATIVE)
+    return SERVING_NATIVE
 
 
 if __name__ == "__main__":
