@@ -17,7 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "libexactattn_cuda.so")
 SOURCES = ["ea_simt.cu", "ea_tc.cu", "ea_decode.cu", "ea_api.cu", "ea_synth.cu", "ea_noalloc.cu", "ea_cache.cu",
-           "ea_selftest.cu", "ea_nccl.cu", "ea_plan.cu", "ea_rope.cu", "ea_tree.cu", "ea_logits.cu"]
+           "ea_selftest.cu", "ea_nccl.cu", "ea_plan.cu", "ea_rope.cu", "ea_tree.cu",
+           "ea_tree_tc.cu", "ea_logits.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
 HEADERS = [os.path.join(HERE, "..", "include", f) for f in ("exactattn_cuda.h", "exactattn_serving.h")]
 

@@ -157,7 +157,6 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
   uint32_t* sums = (uint32_t*)(pool + S::POOL);
   __shared__ uint64_t scratch[32];
   __shared__ float join_m[WARPS][ROWS], join_l[WARPS][ROWS];
-  __shared__ float weights[WARPS][ROWS][17];  // the slow path's weights, -1: not seen
   Schedule<ROWS, KT> sch;
   sch.build(a, sums, scratch);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -310,29 +309,17 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
         }
       }
       if (__any_sync(0xffffffffu, bad)) {
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int kk = nt * 8 + 2 * (lane & 3) + (e & 1);
-            weights[warp][lane / 4 + 8 * (e >> 1)][kk] =
-                sees(a, it, tok[e >> 1], key0 + kk, (okm >> kk) & 1) ? s[nt][e] : -1.0f;
-          }
-        __syncwarp();
         for (int kk = 0; kk < 16; ++kk) {
+          const bool see0 = sees(a, it, tok[0], key0 + kk, (okm >> kk) & 1), see1 = sees(a, it, tok[1], key0 + kk, (okm >> kk) & 1);
 #pragma unroll
           for (int nn = 0; nn < DP / 8; ++nn)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int c = nn * 8 + 2 * (lane & 3) + e;
-              const T v = *(const T*)(pool + (vb - smem_addr(pool)) + swz<DP>(kk, c >> 3) + (c & 7) * 2);
-              const float f = to_f(v);
+              const float f = to_f(*(const T*)(pool + (vb - smem_addr(pool)) + swz<DP>(kk, c >> 3) + (c & 7) * 2));
               if (isfinite(f)) continue;
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const float w = weights[warp][lane / 4 + 8 * half][kk];
-                if (w != -1.0f) o[nn][2 * half + e] += w * f;
-              }
+              if (see0) o[nn][e] += f;
+              if (see1) o[nn][2 + e] += f;
             }
         }
         __syncwarp();
@@ -427,8 +414,18 @@ int check(const ea_tree_attention_t* t) {
   return 0;
 }
 
-int workers_for(const ea_tree_attention_t& t) {
-  const int64_t most = most_units(t, ROWS, KT), fill = 2 * (int64_t)sm_count();
+// Which kernel: query rows per sequence and kv head at most 16 (few_rows_kernel), 128, or more. max_new is a hint,
+// so any choice is right for any lengths.
+struct Choice {
+  int rows, kt, per_sm;
+};
+Choice choose(const ea_tree_attention_t& t) {
+  const int64_t rows = (int64_t)(t.max_new > 0 ? t.max_new : 1) * (t.q_heads / t.kv_heads);
+  if (rows <= ROWS || t.batch > MANY_MAX_SEQS) return {ROWS, KT, 2};
+  return {rows <= 128 ? 128 : 256, 128, 1};
+}
+int workers_for(const ea_tree_attention_t& t, const Choice& c) {
+  const int64_t most = most_units(t, c.rows, c.kt), fill = (int64_t)c.per_sm * sm_count();
   return (int)(most < fill ? (most > 0 ? most : 1) : fill);
 }
 
@@ -441,7 +438,8 @@ extern "C" int64_t ea_tree_attention_workspace(const ea_tree_attention_t* t) {
   using namespace ea::serving;
   if (tree::check(t)) return -1;
   const int dp = t->d <= 64 ? 64 : 128;
-  return (int64_t)tree::workers_for(*t) * 2 * tree::ROWS * (dp + 2) * 4;
+  const tree::Choice c = tree::choose(*t);
+  return (int64_t)tree::workers_for(*t, c) * 2 * c.rows * (dp + 2) * 4;
 }
 
 extern "C" int ea_tree_attention_cuda(const ea_tree_attention_t* t, void* stream) {
@@ -462,8 +460,10 @@ extern "C" int ea_tree_attention_cuda(const ea_tree_attention_t* t, void* stream
   a.by_page = fast_div((uint32_t)t->page_size);
   a.by_group = fast_div((uint32_t)a.group);
   a.dp = t->d <= 64 ? 64 : 128;
-  a.workers = tree::workers_for(*t);
+  const tree::Choice c = tree::choose(*t);
+  a.workers = tree::workers_for(*t, c);
   cudaStream_t st = (cudaStream_t)stream;
+  if (c.rows > tree::ROWS) return tree::launch_many(a, c.rows == 256, st);
   if (t->dtype == EA_BF16)
     return a.dp == 64 ? tree::launch<__nv_bfloat16, 64>(a, st) : tree::launch<__nv_bfloat16, 128>(a, st);
   return a.dp == 64 ? tree::launch<__half, 64>(a, st) : tree::launch<__half, 128>(a, st);

@@ -108,7 +108,11 @@ __device__ __forceinline__ float* slot_of(const Args& a, int slot, int rows) {
   return (float*)a.t.workspace + (int64_t)slot * rows * (a.dp + 2);
 }
 
-// Adds up the partials of the item that share `blockIdx.x` left unfinished. Thread (row group, channel).
+// Kernel for more than 16 rows per kv head (ea_tree_tc.cu): 256-row items with `pair`, else 128-row ones.
+constexpr int MANY_MAX_SEQS = 6000;  // what its shared memory has room for
+int launch_many(const Args& a, bool pair, cudaStream_t st);
+
+// Adds up the partials of the item that share blockIdx.x left unfinished, 16 rows a block (blockIdx.y).
 template <typename T, int ROWS, int KT, int THREADS>
 __global__ void __launch_bounds__(THREADS) combine_kernel(Args a) {
   extern __shared__ uint32_t sums[];
@@ -124,13 +128,13 @@ __global__ void __launch_bounds__(THREADS) combine_kernel(Args a) {
   if (begin < lo || end <= hi) return;  // begun earlier, or finished here
   int last = w;
   while (sch.share(last + 1) < end) ++last;
-  const int rows = min(ROWS, it.new_tokens * a.group - it.m * ROWS);
+  const int r0 = blockIdx.y * 16, rows = min(16, min(ROWS, it.new_tokens * a.group - it.m * ROWS) - r0);
   const int stride = ROWS * (a.dp + 2);
   const float* first = slot_of(a, 2 * w + 1, ROWS);
   const float* rest = slot_of(a, 2 * w, ROWS);  // share w' > w: rest + (w' - w) * 2 * stride
   const int cols = a.dp;
   for (int e = threadIdx.x; e < rows * cols; e += THREADS) {
-    const int r = e / cols, c = e - r * cols;
+    const int r = r0 + e / cols, c = e % cols;
     float m = first[ROWS * a.dp + r];
     for (int i = 1; i <= last - w; ++i) m = fmaxf(m, rest[(int64_t)i * 2 * stride + ROWS * a.dp + r]);
     const float base = m == -INFINITY ? 0.0f : m;

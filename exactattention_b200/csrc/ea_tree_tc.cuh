@@ -1,0 +1,606 @@
+// Tree attention for many query rows per kv head on the 5th-generation tensor cores (tcgen05): 128-row tiles.
+//
+// Per block one work item at a time: its query rows (tokens x the heads of a group) in shared memory, key and
+// value tiles of 128 keys streamed through a ring of buffers. Two softmax slots of 128 threads (a thread a row)
+// take turns on the tensor core:
+//   PAIR  = true : the item has 256 rows, slot s owns rows 128 s .. and both use every key tile (half the
+//                  traffic from L2 per row);
+//   PAIR  = false: the item has 128 rows and slot s takes the key tiles of parity s; the two partial results are
+//                  joined at the item's end.
+// A slot's cycle: S = Q K^T into tensor memory (SS form, both operands K-major, 128-byte swizzle) -> row maximum,
+// weights 2^(alpha s - m) and their sum in registers -> the weights as 16-bit numbers into tensor memory over S ->
+// O += P V (A from tensor memory, V with its channels as the MN-major dimension). While one slot computes
+// weights the other's products run: at 128 x 128 keys x 128 channels each of the two products takes about 512
+// cycles of the tensor pipe and the 16384 exponentials 1024 cycles of the special-function pipe.
+// The MMA thread issues PV(t) and then QK of the slot's next tile, so one arrival per cycle tells the slot that its
+// scores are there and that O is at rest: the rescale of O needs no wait of its own. It happens only when a row's
+// maximum grew by more than 8 (weights stay below 2^8, far from any overflow, and nothing is lost: the sum and O
+// share the reference).
+// Weights are rounded to the cache's type for the product (relative error 2^-9 for bf16, 2^-12 for fp16, of
+// random sign, about the rounding of the output itself); their sum takes them unrounded.
+#pragma once
+#include "ea_tcgen05.cuh"
+#include "ea_tree.cuh"
+
+namespace ea {
+namespace serving {
+namespace tree {
+namespace many {
+
+using namespace ea::tc;
+
+constexpr int KT = 128, TILE = 128, THREADS = 512;
+constexpr int SLOT_THREADS = 128, LOADERS = 128;
+constexpr uint32_t COL_S = 0, COL_O = 256;  // slot s: + 128 s
+constexpr int PAGE_RING = 16;
+
+template <int DP, bool PAIR>
+struct Cfg {
+  static constexpr int ROWS = PAIR ? 256 : 128;
+  static constexpr int BUF = KT * DP * 2;  // a tile of keys or values
+  static constexpr int NBUF = DP == 64 ? 8 : PAIR ? 4 : 5;
+  static constexpr int QBYTES = ROWS * DP * 2;
+  static constexpr int SMEM = QBYTES + NBUF * BUF + 1024;  // + alignment; the schedule's sums follow
+};
+
+struct Shared {
+  uint64_t full[8], empty[8], s_full[2], p_ready[2], q_full, done;
+  uint64_t scratch[32];
+  uint32_t tmem;
+  uint32_t page_ok[PAGE_RING][4];
+  int dirty[2];
+  float m[2][TILE], l[2][TILE];
+};
+
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
+  return (1u << 4) | ((std::is_same<T, __half>::value ? 0u : 1u) << 7) | ((std::is_same<T, __half>::value ? 0u : 1u) << 10) |
+         ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
+}
+
+// shared-memory descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart; `lbo`: distance between the 64-element
+// blocks of an MN-major operand
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024u >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool try_now(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done;
+}
+
+#define EA_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define EA_I8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+// 32 consecutive columns of this thread's lane
+__device__ __forceinline__ void ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : EA_R8(v, 0), EA_R8(v, 8), EA_R8(v, 16), EA_R8(v, 24)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      EA_I8(v, 0), EA_I8(v, 8), EA_I8(v, 16), EA_I8(v, 24)
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *(const uint32_t*)&h;
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *(const uint32_t*)&h;
+}
+template <int REGS, bool INC>
+__device__ __forceinline__ void set_regs() {
+  if (INC) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+// byte offset of (row, 16-byte piece) in a tile of `rows` rows of 64-channel blocks, 128-byte swizzle
+__device__ __forceinline__ uint32_t tile_off(int row, int piece, int rows) {
+  return (uint32_t)((piece >> 3) * rows * 128 + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+}
+
+// Bits of keys k0 .. k0 + 31 that token i of the item sees; tile pages aside.
+__device__ __forceinline__ uint32_t seen_word(const Args& a, const Item& it, int i, int k0) {
+  const int ctx = it.len - it.new_tokens, j0 = k0 - ctx;
+  const auto low = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
+  uint32_t bits;
+  if (j0 <= -32) {
+    bits = 0xFFFFFFFFu;
+  } else if (!a.t.tree_mask) {
+    bits = low(i + 1 - j0);
+  } else {
+    const uint32_t* row = (const uint32_t*)a.t.tree_mask + (int64_t)(it.q0 + i) * a.t.mask_words;
+    const auto word = [&](int w) { return w >= 0 && w < a.t.mask_words ? row[w] : 0u; };
+    if (j0 >= 0) bits = __funnelshift_r(word(j0 >> 5), word((j0 >> 5) + 1), j0 & 31);
+    else bits = (word(0) << -j0) | low(-j0);
+  }
+  return bits & low(it.len - k0);
+}
+
+template <typename T>
+__device__ __forceinline__ bool pair_not_finite(uint32_t v) {
+  constexpr uint32_t EXP = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return (v & EXP) == EXP || (v & EXP << 16) == EXP << 16;
+}
+
+// Zeroes the infinities and NaN of one row of a value tile; whether there were any.
+template <typename T, int DP>
+__device__ __noinline__ bool clean_row(uint8_t* buf, int row) {
+  constexpr uint32_t EXP = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  bool any = false;
+  for (int p = 0; p < DP / 8; ++p) {
+    uint32_t* w = (uint32_t*)(buf + tile_off(row, p, KT));
+    for (int e = 0; e < 4; ++e) {
+      uint32_t v = w[e];
+      if (!pair_not_finite<T>(v)) continue;
+      any = true;
+      if ((v & EXP) == EXP) v &= 0xFFFF0000u;
+      if ((v & EXP << 16) == EXP << 16) v &= 0xFFFFu;
+      w[e] = v;
+    }
+  }
+  return any;
+}
+
+// Adds to acc (channels c0 ..) the infinities and NaN of the values of drafted keys first .. last - 1 that token i sees.
+template <typename T, int N>
+__device__ __noinline__ void add_not_finite(const Args& a, const Item& it, int i, int first, int last, int c0, float* acc) {
+  for (int k = max(first, it.len - it.new_tokens); k < min(last, it.len); ++k) {
+    if (k < 0 || !((seen_word(a, it, i, k)) & 1)) continue;
+    const uint32_t col = div_by((uint32_t)k, a.by_page);
+    const int page = a.t.page_table[it.b * a.t.table_stride + col];
+    if (page < 0 || page >= a.t.num_pages) continue;
+    const T* v = (const T*)a.t.v_cache + (int64_t)page * a.t.v_page_stride + it.h * a.t.v_head_stride +
+                 (k - (int64_t)col * a.t.page_size) * a.t.v_row_stride;
+    for (int c = 0; c < N; ++c) {
+      if (c0 + c >= a.t.d) break;
+      const float f = to_f(v[c0 + c]);
+      if (!isfinite(f)) acc[c] += f;
+    }
+  }
+}
+
+template <typename T, int DP, bool PAIR>
+__global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
+  using C = Cfg<DP, PAIR>;
+  constexpr int ROWS = C::ROWS, NBUF = C::NBUF, BUF = C::BUF;
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared sh;
+  uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* qbuf = base;
+  uint8_t* ring = base + C::QBYTES;
+  uint32_t* sums = (uint32_t*)(raw + C::SMEM);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  Schedule<ROWS, KT> sch;
+  sch.build(a, sums, sh.scratch);
+  if (tid == 0) {
+    for (int i = 0; i < NBUF; ++i) mbar_init(&sh.full[i], LOADERS), mbar_init(&sh.empty[i], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], SLOT_THREADS);
+    mbar_init(&sh.q_full, 2 * SLOT_THREADS);
+    mbar_init(&sh.done, 1);
+    sh.dirty[0] = sh.dirty[1] = 0;
+  }
+  if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = sh.tmem;
+  uint32_t pos = sch.share(blockIdx.x);
+  const uint32_t end = sch.share(blockIdx.x + 1);
+  bool alive = true;  // false once a bounded wait gave up: no more waits, products or copies; the rows become NaN
+
+  if (warp >= 12) {
+    // ---- loaders: every thread copies 16-byte pieces of every tile, in the order the products use them
+    set_regs<64, false>();
+    const int w4 = warp - 12, key_lane = w4 * 32 + lane;
+    uint32_t cnt = 0, pending = 0, signalled = 0, tile0 = 0;  // tile0: tiles of earlier items
+    const auto retire = [&]() {  // waits for the oldest tile in flight and hands it over
+      switch (pending) {
+        case 1: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+        case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+        case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+        case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        case 5: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+        case 6: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+        case 7: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
+      }
+      fence_async_smem();
+      arrive(&sh.full[signalled % NBUF]);
+      ++signalled, --pending;
+    };
+    while (pos < end && alive) {
+      const Item it = sch.item(a, pos, end);
+      pos += it.kt1 - it.kt0;
+      const int n = it.kt1 - it.kt0;
+      const auto page_of = [&](int t) {
+        const int key = (it.kt0 + t) * KT + key_lane;
+        if (t >= n || key >= it.len) return -1;
+        const int p = a.t.page_table[it.b * a.t.table_stride + div_by((uint32_t)key, a.by_page)];
+        return p >= 0 && p < a.t.num_pages ? p : -1;
+      };
+      const auto load = [&](int t, int page, bool value) {
+        const uint32_t b = cnt % NBUF;
+        if (cnt >= NBUF) {
+          const uint32_t parity = (cnt / NBUF - 1) & 1;
+          while (pending && !__all_sync(0xffffffffu, try_now(&sh.empty[b], parity))) retire();
+          alive = __all_sync(0xffffffffu, mbar_wait(&sh.empty[b], parity));
+          if (!alive) return;
+        }
+        if (pending == 7) retire();
+        if (!value) {
+          const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
+          if (lane == 0) sh.page_ok[(tile0 + t) % PAGE_RING][w4] = ok;
+        }
+        const uint32_t dst = smem_u32(ring + b * BUF);
+        const T* src = (const T*)(value ? a.t.v_cache : a.t.k_cache) + it.h * (value ? a.t.v_head_stride : a.t.k_head_stride);
+        const int64_t ps = value ? a.t.v_page_stride : a.t.k_page_stride, rs = value ? a.t.v_row_stride : a.t.k_row_stride;
+        const int key0 = (it.kt0 + t) * KT + w4 * 32;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int r = q * 4 + lane / 8;
+          const int pg = __shfl_sync(0xffffffffu, page, r);
+          const int key = key0 + r;
+          const int64_t off = pg >= 0 ? key - (int64_t)div_by((uint32_t)key, a.by_page) * a.t.page_size : 0;
+          const T* row = src + (pg >= 0 ? pg : 0) * ps + off * rs;
+#pragma unroll
+          for (int c = 0; c < DP / 64; ++c) {
+            const int piece = c * 8 + (lane & 7);
+            const bool in = pg >= 0 && piece * 8 < a.t.d;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + tile_off(w4 * 32 + r, piece, KT)),
+                         "l"(in ? (const void*)(row + piece * 8) : (value ? a.t.v_cache : a.t.k_cache)), "r"(in ? 16 : 0)
+                         : "memory");
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ++cnt, ++pending;
+      };
+      // order of use: PAIR K0, then V(t), K(t + 1); else K0, K1, then V(t), K(t + 2)
+      constexpr int AHEAD = PAIR ? 1 : 2;
+      int page[AHEAD + 1], next = page_of(AHEAD);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) page[i] = page_of(i);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (i < n && alive) load(i, page[i], false);
+      for (int t = 0; t < n && alive; ++t) {
+        page[AHEAD] = next;
+        next = page_of(t + AHEAD + 1);
+        load(t, page[0], true);
+        if (t + AHEAD < n && alive) load(t + AHEAD, page[AHEAD], false);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) page[i] = page[i + 1];
+      }
+      tile0 += n;
+    }
+    while (pending) retire();
+  } else if (warp >= 8) {
+    // ---- the MMA thread
+    set_regs<64, false>();
+    if (warp == 8 && lane == 0) {
+      constexpr uint32_t QK = idesc<T>(KT, false), PV = idesc<T>(DP, true);
+      uint32_t cnt = 0, items = 0, np[2] = {0, 0};
+      const uint32_t qa = smem_u32(qbuf), ra = smem_u32(ring);
+      const auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (alive && !mbar_wait(bar, parity)) alive = false;
+      };
+      while (pos < end && alive) {
+        const Item it = sch.item(a, pos, end);
+        pos += it.kt1 - it.kt0;
+        const int n = it.kt1 - it.kt0;
+        const bool two = !PAIR || it.new_tokens * a.group - it.m * ROWS > TILE;
+        wait(&sh.q_full, items & 1);
+        ++items;
+        const auto buf_full = [&](uint32_t c) { wait(&sh.full[c % NBUF], (c / NBUF) & 1); };
+        const auto qk = [&](int slot, uint32_t c) {
+          if (!alive) return;
+          const uint32_t qs = qa + (PAIR ? slot * TILE * 128 : 0), kb = ra + (c % NBUF) * BUF;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            mma_ss(tmem + COL_S + slot * 128, desc_sw128(qs + (k >> 2) * ROWS * 128 + (k & 3) * 32, 16),
+                   desc_sw128(kb + (k >> 2) * KT * 128 + (k & 3) * 32, 16), QK, k > 0);
+        };
+        const auto pv = [&](int slot, uint32_t c, bool acc) {
+          if (!alive) return;
+          const uint32_t vb = ra + (c % NBUF) * BUF;
+#pragma unroll
+          for (int k = 0; k < KT / 16; ++k)
+            mma_ts(tmem + COL_O + slot * 128, tmem + COL_S + slot * 128 + k * 8, desc_sw128(vb + k * 2048, KT * 128), PV,
+                   acc || k > 0);
+        };
+        const auto commit = [&](uint64_t* bar) {
+          if (alive) mma_commit(smem_u32(bar));
+        };
+        const auto weights = [&](int slot) {
+          wait(&sh.p_ready[slot], np[slot]++ & 1);
+          fence_after_sync();
+        };
+        if (PAIR) {
+          buf_full(cnt);
+          qk(0, cnt);
+          commit(&sh.s_full[0]);
+          if (two) qk(1, cnt);
+          commit(&sh.s_full[1]);
+          commit(&sh.empty[cnt % NBUF]);
+          ++cnt;
+          for (int t = 0; t < n && alive; ++t) {
+            const bool more = t + 1 < n;
+            const uint32_t cv = cnt, ck = cnt + 1;
+            weights(0);
+            buf_full(cv);
+            pv(0, cv, t > 0);
+            if (more) buf_full(ck), qk(0, ck);
+            commit(&sh.s_full[0]);
+            if (two) weights(1), pv(1, cv, t > 0);
+            commit(&sh.empty[cv % NBUF]);
+            if (more) {
+              if (two) qk(1, ck);
+              commit(&sh.empty[ck % NBUF]);
+            }
+            if (two) commit(&sh.s_full[1]);
+            cnt += more ? 2 : 1;
+          }
+        } else {
+          for (int t = 0; t < 2; ++t) {
+            if (t < n) {
+              buf_full(cnt);
+              qk(t, cnt);
+              commit(&sh.empty[cnt % NBUF]);
+              ++cnt;
+            }
+            commit(&sh.s_full[t]);
+          }
+          for (int t = 0; t < n && alive; ++t) {
+            const int slot = t & 1;
+            weights(slot);
+            buf_full(cnt);
+            pv(slot, cnt, t > 1);
+            commit(&sh.empty[cnt % NBUF]);
+            ++cnt;
+            if (t + 2 < n) {
+              buf_full(cnt);
+              qk(slot, cnt);
+              commit(&sh.empty[cnt % NBUF]);
+              ++cnt;
+            }
+            commit(&sh.s_full[slot]);
+          }
+        }
+      }
+      // what has been issued completes before the block frees its tensor memory
+      mma_commit(smem_u32(&sh.done));
+      mbar_wait(&sh.done, 0);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax slots
+    set_regs<192, true>();
+    const int slot = warp >> 2, r = tid & (TILE - 1);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lanes + COL_S + slot * 128, o_addr = lanes + COL_O + slot * 128;
+    const float alpha = fabsf(a.t.alpha);
+    const uint32_t flip = a.t.alpha < 0 ? 0x80008000u : 0u, keep = a.t.alpha == 0 ? 0u : 0xFFFFFFFFu;
+    const float scale_s = a.t.alpha == 0 ? 1.0f : alpha;
+    uint32_t ns = 0, first = 0;  // phases of s_full seen; ring position of the item's first tile
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+    };
+    while (pos < end) {
+      const Item it = sch.item(a, pos, end);
+      pos += it.kt1 - it.kt0;
+      const int n = it.kt1 - it.kt0, ctx = it.len - it.new_tokens;
+      const int all_rows = it.new_tokens * a.group - it.m * ROWS;
+      const int rows = min(TILE, all_rows - (PAIR ? slot * TILE : 0));  // of this slot's tile; may be <= 0 for PAIR
+      const int R = it.m * ROWS + (PAIR ? slot * TILE : 0) + min(r, max(rows, 1) - 1);
+      const int tok = (int)div_by((uint32_t)R, a.by_group);
+      // the slot's query rows into shared memory (PAIR: its own tile; else half of the pieces each)
+      if (rows > 0) {
+        const T* q = (const T*)a.t.q + (int64_t)(it.q0 + tok) * a.t.q_stride +
+                     (int64_t)(it.h * a.group + R - tok * a.group) * a.t.q_head_stride;
+        constexpr int PIECES = PAIR ? DP / 8 : DP / 16;
+        const int p0 = PAIR ? 0 : slot * PIECES;
+        uint4 x[PIECES];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+          x[p] = (p0 + p) * 8 < a.t.d ? *(const uint4*)(q + (p0 + p) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+          x[p].x = (x[p].x & keep) ^ flip, x[p].y = (x[p].y & keep) ^ flip;
+          x[p].z = (x[p].z & keep) ^ flip, x[p].w = (x[p].w & keep) ^ flip;
+          *(uint4*)(qbuf + tile_off((PAIR ? slot * TILE : 0) + r, p0 + p, ROWS)) = x[p];
+        }
+      }
+      if (r == 0) sh.dirty[slot] = 0;
+      fence_async_smem();
+      fence_before_sync();
+      arrive(&sh.q_full);
+
+      const bool warp_rows = (r & ~31) < rows;
+      const int tiles = PAIR ? (rows > 0 ? n : 0) : (n + 1 - slot) / 2;
+      float m = -INFINITY, l = 0.0f;
+      for (int i = 0; i < tiles; ++i) {
+        const int t = PAIR ? i : 2 * i + slot;
+        const int key0 = (it.kt0 + t) * KT;
+        wait(&sh.s_full[slot], ns++ & 1);
+        fence_after_sync();
+        const uint32_t* ok = sh.page_ok[(first / 2 + t) % PAGE_RING];
+        const bool masked = key0 + KT > ctx || (ok[0] & ok[1] & ok[2] & ok[3]) != 0xFFFFFFFFu;
+        if (warp_rows && alive) {
+          float s[KT];
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c) ld32(s_addr + c * 32, (uint32_t*)s + c * 32);
+          tmem_wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c) {
+              const uint32_t vis = seen_word(a, it, tok, key0 + c * 32) & ok[c];
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((vis >> e) & 1)) s[c * 32 + e] = -INFINITY;
+            }
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < KT; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_s;
+          const bool grow = top > m + 8.0f || (m == -INFINITY && top != -INFINITY);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float f = grow ? (m == -INFINITY ? 0.0f : ex2(m - top)) : 1.0f;
+            if (grow) m = top;
+            l *= f;
+            if (i > 0) {
+#pragma unroll
+              for (int c = 0; c < DP / 32; ++c) {
+                uint32_t o[32];
+                ld32(o_addr + c * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                st32(o_addr + c * 32, o);
+              }
+            }
+          }
+          const float ref = m == -INFINITY ? 0.0f : m;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float x = ex2(fmaf(s[c * 64 + 2 * e], scale_s, -ref)), y = ex2(fmaf(s[c * 64 + 2 * e + 1], scale_s, -ref));
+              sum[e & 1] += x, sum[2 + (e & 1)] += y;
+              p[e] = pack2(x, y, T());
+            }
+            st32(s_addr + c * 32, p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        // drafted keys: their infinities and NaN may not meet the zero weight of a row that does not see them
+        if (key0 + KT > ctx && (!PAIR || slot == 0)) {
+          const uint32_t c = first + (PAIR ? 1 + 2 * t : n == 1 ? 1 : 2 + t + min(t, n - 2));
+          wait(&sh.full[c % NBUF], (c / NBUF) & 1);
+          if (alive && clean_row<T, DP>(ring + (c % NBUF) * BUF, r) && key0 + r < it.len) sh.dirty[slot] = 1;
+          fence_async_smem();
+        }
+        fence_before_sync();
+        arrive(&sh.p_ready[slot]);
+      }
+      wait(&sh.s_full[slot], ns++ & 1);  // the slot's products are done
+      fence_after_sync();
+      first += 2 * n;
+
+      // join the slots (PAIR: each has rows of its own) and write the rows
+      if (!alive) l = NAN;
+      const bool whole = it.kt0 == 0 && it.kt1 == it.tiles;
+      float ml[2] = {m, m}, ll[2] = {l, 0.0f};
+      if (!PAIR) {
+        sh.m[slot][r] = m, sh.l[slot][r] = l;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        ml[0] = sh.m[0][r], ml[1] = sh.m[1][r], ll[0] = sh.l[0][r], ll[1] = sh.l[1][r];
+      } else {
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      const bool dirty = sh.dirty[0] || sh.dirty[1];
+      const float mm = fmaxf(ml[0], ml[1]), ref = mm == -INFINITY ? 0.0f : mm;
+      const float f0 = exp2f(ml[0] - ref), f1 = PAIR || n < 2 ? 0.0f : exp2f(ml[1] - ref);
+      const float lsum = ll[0] * f0 + ll[1] * (PAIR ? 0.0f : exp2f(ml[1] - ref));
+      const bool mine = r < rows;
+      const int64_t head = (int64_t)(it.q0 + tok) * a.t.q_heads + it.h * a.group + (R - tok * a.group);
+      const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+      float* part = slot_of(a, 2 * blockIdx.x + (it.kt0 == 0 ? 1 : 0), ROWS);
+      const int pr = (PAIR ? slot * TILE : 0) + r;
+      constexpr int COLS = PAIR ? DP : DP / 2;
+      const int c0 = PAIR ? 0 : slot * COLS;
+      if (warp_rows) {
+#pragma unroll
+        for (int c = 0; c < COLS / 32; ++c) {
+          uint32_t u[32];
+          float o[32];
+          ld32(lanes + COL_O + (PAIR ? slot * 128 : 0) + c0 + c * 32, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(u[e]) * f0;
+          if (!PAIR && n > 1) {
+            ld32(lanes + COL_O + 128 + c0 + c * 32, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
+          }
+          const int ch = c0 + c * 32;
+          if (mine && dirty) add_not_finite<T, 32>(a, it, tok, it.kt0 * KT, it.kt1 * KT, ch, o);
+          if (mine && whole) {
+            T* dst = (T*)a.t.out + head * a.t.d + ch;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              uint4 y;
+              uint32_t* yw = (uint32_t*)&y;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) yw[e] = pack2(o[p * 8 + 2 * e] * inv, o[p * 8 + 2 * e + 1] * inv, T());
+              if (ch + p * 8 < a.t.d) *(uint4*)(dst + p * 8) = y;
+            }
+          } else if (mine) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *(float4*)(part + (int64_t)pr * DP + ch + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+          __syncwarp();
+        }
+      }
+      if (mine && (PAIR || slot == 0)) {
+        if (whole) {
+          if (a.t.lse) a.t.lse[head] = lsum == 0.0f ? -INFINITY : mm + log2f(lsum);
+        } else {
+          part[ROWS * DP + pr] = mm, part[ROWS * (DP + 1) + pr] = lsum;
+        }
+      }
+      fence_before_sync();
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // m, l and dirty are read; O is free
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  if (warp == 8) tmem_free(tmem, 512);
+}
+
+}  // namespace many
+}  // namespace tree
+}  // namespace serving
+}  // namespace ea
