@@ -1,13 +1,14 @@
 // Penalties for repeated tokens, biases and grammar masks on logits (ea_process_logits_cuda).
 //
-// Bound by HBM: a row's logits are read once and written once. A block owns a chunk of one row's
-// vocabulary. What changes a token beyond its mask bit is kept in a table of one 32-bit word per token
-// of the chunk in shared memory, built from the row's history, path and bias list:
+// Bound by HBM: a row's logits are read once and written once. A block owns a chunk of one row's vocabulary. It
+// streams the chunk through, setting what the mask forbids to -inf, and corrects the few tokens that penalties or
+// biases change afterwards. Which these are is in a table of one 32-bit word per token of the chunk in shared memory,
+// built from the row's history, path and bias list while the first logits are on their way:
 //   bits 0-19 how often the token was generated, bits 20-30 which bias entry it has first
 //   (EA_LOGITS_MAX_BIASES - entry, 0: none), bit 31 whether the prompt holds it.
-// The words are integers, so the order of the atomics cannot change them. The first logits are loaded
-// before the table is built, so their latency overlaps the scan of the history. Rows without penalties
-// and biases build no table.
+// The words are integers, so the order of the atomics cannot change them. The corrections walk over the same lists:
+// who swaps a token's nonzero word for zero corrects the token. So the dense part reads no table, and the cost of the
+// sparse part follows the lists' lengths. Rows without penalties and biases build no table.
 #include "ea_serving.cuh"
 
 namespace ea {
@@ -32,7 +33,7 @@ struct Row {
 };
 
 // The row's rule for one token whose table word is not zero.
-__device__ __noinline__ float adjust(float x, uint32_t w, int token, const Row& r, int num_biases) {
+__device__ __forceinline__ float adjust(float x, uint32_t w, int token, const Row& r, int num_biases) {
   const uint32_t cnt = w & COUNT, code = (w >> CODE_SHIFT) & 0x7FFu;
   if (cnt || (w & PROMPT)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
   x = __fsub_rn(x, __fmul_rn(r.freq, (float)cnt));
@@ -48,8 +49,8 @@ __device__ __noinline__ float adjust(float x, uint32_t w, int token, const Row& 
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(THREADS) logits_kernel(ea_process_logits_t a, int chunk, FastDiv by_chunks,
-                                                         int chunks) {
+__global__ void __launch_bounds__(THREADS, 2) logits_kernel(ea_process_logits_t a, int chunk, FastDiv by_chunks,
+                                                            int chunks) {
   using P = Pack<T, VEC>;
   extern __shared__ uint4 table4[];
   uint32_t* table = (uint32_t*)table4;
@@ -80,54 +81,57 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(ea_process_logits_t a, 
   r.rep = real && a.repetition ? a.repetition[b] : 1.0f;
   r.freq = real && a.frequency ? a.frequency[b] : 0.0f;
   r.pres = real && a.presence ? a.presence[b] : 0.0f;
-  r.ids = a.bias_ids + (int64_t)(real ? b : 0) * a.num_biases;
-  r.vals = a.bias_values + (int64_t)(real ? b : 0) * a.num_biases;
-  r.dup = false;
   const bool counts = real && (r.rep != 1.0f || r.freq != 0.0f || r.pres != 0.0f) && (a.history || a.draft_tokens);
   const bool biased = real && a.num_biases > 0;
   const bool tabled = counts || biased;
+  // the chunk's tokens, and the lists: history, path (drafted tokens), biases
+  const uint32_t lo = (uint32_t)max(v0, 0), span = (uint32_t)(min(a.vocab, v0 + chunk)) - lo;
+  int n_hist = 0, n_prompt = 0, n_path = 0;
+  const int32_t *hist = nullptr, *path = nullptr;
+  const uint32_t* seen = nullptr;
   if (tabled) {
-    for (int i = tid; i < chunk / 4; i += THREADS) table4[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) dup = 0;
-    __syncthreads();
-    const uint32_t lo = (uint32_t)max(v0, 0), span = (uint32_t)(min(a.vocab, v0 + chunk)) - lo;
-    uint32_t* at = table + ((int)lo - v0);
     if (counts && a.history) {
-      const int n = min(max(a.history_lens[b], 0), a.max_history);
-      const int np = a.prompt_lens ? min(max(a.prompt_lens[b], 0), n) : 0;
-      const int32_t* h = a.history + (int64_t)b * a.history_stride;
-      for (int i = tid; i < n; i += THREADS) {
-        const uint32_t t = (uint32_t)h[i] - lo;
-        if (t < span) {
-          if (i < np) atomicOr(at + t, PROMPT);
-          else atomicAdd(at + t, 1u);
-        }
-      }
+      n_hist = min(max(a.history_lens[b], 0), a.max_history);
+      n_prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), n_hist) : 0;
+      hist = a.history + (int64_t)b * a.history_stride;
     }
     if (counts && a.draft_tokens) {
       const int64_t q0 = a.q_start[b], q1 = min((int64_t)a.q_start[b + 1], a.rows);
       if (q0 >= 0 && q0 < q1) {
-        const int n = (int)min(q1 - q0, (int64_t)(a.tree_mask ? a.tree_words * 32 : row - q0 + 1));
-        for (int j = tid; j < min(n, EA_LOGITS_MAX_PATH); j += THREADS) {
-          if (a.tree_mask && !((a.tree_mask[row * a.tree_words + (j >> 5)] >> (j & 31)) & 1)) continue;
-          const uint32_t t = (uint32_t)a.draft_tokens[q0 + j] - lo;
-          if (t < span) atomicAdd(at + t, 1u);
-        }
+        n_path = (int)min(min(q1 - q0, (int64_t)(a.tree_mask ? a.tree_words * 32 : row - q0 + 1)), (int64_t)EA_LOGITS_MAX_PATH);
+        path = a.draft_tokens + q0;
+        if (a.tree_mask) seen = (const uint32_t*)a.tree_mask + row * a.tree_words;
       }
     }
+    r.ids = a.bias_ids + (int64_t)b * a.num_biases;
+    r.vals = a.bias_values + (int64_t)b * a.num_biases;
+    for (int i = tid; i < (int)(span + 3) / 4; i += THREADS) table4[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) dup = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < n_hist; i += THREADS) {
+      const uint32_t t = (uint32_t)hist[i] - lo;
+      if (t < span) {
+        if (i < n_prompt) atomicOr(table + t, PROMPT);
+        else atomicAdd(table + t, 1u);
+      }
+    }
+    for (int j = tid; j < n_path; j += THREADS) {
+      if (seen && !((seen[j >> 5] >> (j & 31)) & 1)) continue;
+      const uint32_t t = (uint32_t)path[j] - lo;
+      if (t < span) atomicAdd(table + t, 1u);
+    }
+    __syncthreads();
     if (biased) {
-      __syncthreads();
       for (int e = tid; e < a.num_biases; e += THREADS) {
         const uint32_t t = (uint32_t)r.ids[e] - lo;
         if (t < span) {
           const uint32_t code = (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT;
-          const uint32_t old = atomicMax(at + t, (at[t] & (PROMPT | COUNT)) | code);
+          const uint32_t old = atomicMax(table + t, (table[t] & (PROMPT | COUNT)) | code);
           if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
         }
       }
     }
-    __syncthreads();
-    r.dup = dup != 0;
   }
 
   for (int i0 = 0; i0 < chunk; i0 += UNROLL * THREADS * VEC) {
@@ -148,24 +152,13 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(ea_process_logits_t a, 
         for (int e = 0; e < VEC; ++e)
           if (v + e >= 0 && v + e < a.vocab) x[j].v[e] = src[v + e];
       }
-      if (tabled) {
-        uint32_t w[VEC], any = 0;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) w[e] = table[i + e], any |= w[e];
-        if (any) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (w[e]) x[j].v[e] = from_f<T>(adjust(to_f(x[j].v[e]), w[e], v + e, r, a.num_biases));
-        }
-      }
       if (bits) {
-        // bit e: token v + e is allowed; the piece may lie in two words
+        // bit e of `no`: token v + e is forbidden; the piece may lie in two words
         const int first = max(v, 0), last = min(v + VEC, a.vocab) - 1;
-        const uint32_t w0 = bits[first >> 5], w1 = bits[last >> 5];
-        const uint32_t ok = __funnelshift_r(w0, w1, first & 31);
+        uint32_t no = ~__funnelshift_r(bits[first >> 5], bits[last >> 5], first & 31) << (first - v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-          if (v + e >= first && v + e <= last && !((ok >> (v + e - first)) & 1)) x[j].v[e] = from_f<T>(-INFINITY);
+          if ((no >> e) & 1) x[j].v[e] = from_f<T>(-INFINITY);
       }
       if (whole) {
         *(P*)(dst + v) = x[j];
@@ -176,6 +169,22 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(ea_process_logits_t a, 
       }
     }
   }
+  if (!tabled) return;
+
+  __syncthreads();  // the chunk is written and the table complete
+  r.dup = dup != 0;
+  const auto correct = [&](uint32_t t) {
+    if (t >= span || !table[t]) return;
+    const uint32_t w = atomicExch(table + t, 0u);
+    if (!w) return;
+    const int v = (int)(lo + t);
+    if (bits && !((bits[v >> 5] >> (v & 31)) & 1)) return;
+    dst[v] = from_f<T>(adjust(to_f(src[v]), w, v, r, a.num_biases));
+  };
+  for (int i = tid; i < n_hist; i += THREADS) correct((uint32_t)hist[i] - lo);
+  for (int j = tid; j < n_path; j += THREADS) correct((uint32_t)path[j] - lo);
+  if (biased)
+    for (int e = tid; e < a.num_biases; e += THREADS) correct((uint32_t)r.ids[e] - lo);
 }
 
 template <typename T, int VEC>

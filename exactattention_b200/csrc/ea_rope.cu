@@ -2,11 +2,14 @@
 //   (x, y) -> (x c - y s, y c + x s),
 // optionally with the write of the turned keys and of the values into paged cache rows.
 //
-// Bound by HBM: every element is read once and written once. A thread owns VEC consecutive pairs
-// of one token (two 16-byte pieces of a head), computes their cos / sin once and walks over heads with
-// them, so the trigonometry costs little per byte. The angle is reduced in binary64
-// (turns = position * inv_freq / 2 pi, minus its nearest integer: the product of a 31-bit and a 24-bit
-// number rounds at 2^-53), then sincospif sees an argument in [-1, 1] whatever the position.
+// Bound by HBM: every element is read once and written once. A block takes a few tokens with some or all of their
+// heads; its threads first load their pieces (two 16-byte pieces of a head hold VEC pairs), then compute the
+// cos / sin of the block's tokens into shared memory, one pair of them per (token, frequency), while the loads are
+// under way, and turn and store the pieces. The angle is reduced in 32 bits without loss: turns = position * f with
+// f = inv_freq / 2 pi as a sum of two numbers, the product's rounding error recovered by an FMA, the nearest integer
+// taken off the large part (exact); what is left of 2^-47 relative error is far below a 32-bit result's rounding.
+// sincospif then sees an argument in [-1, 1] whatever the position. Positions of 2^24 and more, which binary32 does
+// not hold, go through binary64.
 #include "ea_serving.cuh"
 
 namespace ea {
@@ -21,104 +24,141 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-struct Plan {
-  int units, turn_units;  // pieces of a head: those that are turned first, then copied ones
-  int groups;             // head groups: thread (token, group, unit) takes heads group, group + groups, ..
-  FastDiv by_units, by_groups, by_page;
-};
-
-// The two pieces of a unit, in elements from the head's start. Turned units hold VEC pairs; a copied unit is
-// the piece at rot + VEC c alone.
-template <int VEC>
-__device__ __forceinline__ void unit_offsets(const ea_rope_t& a, int u, int turn_units, int& o0, int& o1) {
-  if (u < turn_units) {
-    o0 = a.adjacent ? 2 * VEC * u : VEC * u;
-    o1 = a.adjacent ? o0 + VEC : o0 + a.rot / 2;
-  } else {
-    o0 = a.rot + VEC * (u - turn_units);
-    o1 = -1;
+// Keeps the compiler from widening a piece's numbers before this point, which would double the registers it takes
+// across the barrier.
+template <typename T, int VEC>
+__device__ __forceinline__ void keep_packed(Pack<T, VEC>& p) {
+  if constexpr (sizeof(p) == 16) {
+    uint32_t* w = (uint32_t*)&p;
+    asm volatile("" : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]));
   }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(THREADS) rope_kernel(ea_rope_t a, Plan p) {
-  using P = Pack<T, VEC>;
-  const int64_t item = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-  const int per_tok = p.units * p.groups;
-  const int64_t tok = item / per_tok;
-  if (tok >= a.tokens) return;
-  const uint32_t rem = (uint32_t)(item - tok * per_tok);
-  const int grp = (int)div_by(rem, p.by_units), u = (int)(rem - grp * p.units);
-  int o0, o1;
-  unit_offsets<VEC>(a, u, p.turn_units, o0, o1);
-  const bool turn = u < p.turn_units;
+struct Plan {
+  int units, turn_units;        // pieces of a head: those that are turned first, then copied ones
+  int tokens, heads, head_blocks;  // of a block; blocks a token group
+  int all_heads;
+  FastDiv by_units, by_heads, by_half, by_page, by_head_blocks;
+};
 
-  float c[VEC], s[VEC];
-  if (turn) {
+__device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
+  float r;
+  if (abs(pos) < (1 << 24)) {
+    const float c_hi = 0.15915494f;                              // 1 / (2 pi) = c_hi + c_lo
+    const float c_lo = (float)(INV_2PI - (double)0.15915494f);
+    const float f_hi = freq * c_hi, f_lo = fmaf(freq, c_lo, fmaf(freq, c_hi, -f_hi));
+    const float p = (float)pos, t = p * f_hi, e = fmaf(p, f_lo, fmaf(p, f_hi, -t));
+    r = (t - rintf(t)) + e;
+  } else {
+    const double t = (double)pos * (double)freq * INV_2PI;
+    r = (float)(t - rint(t));
+  }
+  float2 cs;
+  sincospif(2.0f * r, &cs.y, &cs.x);
+  if (inverse) cs.y = -cs.y;
+  return cs;
+}
+
+template <typename T, int VEC, int ITEMS>
+__global__ void __launch_bounds__(THREADS, 3) rope_kernel(ea_rope_t a, Plan p) {
+  using P = Pack<T, VEC>;
+  extern __shared__ float2 cs[];  // (tokens, rot / 2)
+  const uint32_t group = div_by(blockIdx.x, p.by_head_blocks);
+  const int64_t tok0 = (int64_t)group * p.tokens;
+  const int h0 = (int)(blockIdx.x - group * p.head_blocks) * p.heads;
+  const int nk = a.q_heads + a.kv_heads, half = a.rot / 2;
+  const int toks = (int)min((int64_t)p.tokens, a.tokens - tok0), heads = min(p.heads, p.all_heads - h0);
+
+  P x[ITEMS], y[ITEMS];
+  T* dst[ITEMS];       // of the first piece; nullptr: nothing to do
+  int first[ITEMS];    // of the piece's cos / sin; -1: copied
+  uint32_t pairs = 0;  // bit i: item i has a second piece
+  const int apart = a.adjacent ? VEC : half;  // from the first piece
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int f = u * VEC + i;
-      const int ax = a.axes ? min(max(a.axes[f], 0), a.num_axes - 1) : 0;
-      const double turns = (double)a.positions[ax * a.axis_stride + tok] * (double)a.inv_freq[f] * INV_2PI;
-      const float r = (float)(turns - rint(turns));
-      sincospif(2.0f * r, &s[i], &c[i]);
-      if (a.inverse) s[i] = -s[i];
-    }
-  }
-  int64_t kdst = 0, vdst = 0;
-  bool store_kv = true;
-  if (a.slot_map) {
-    const int64_t slot = a.slot_map[tok];
-    store_kv = slot >= 0 && slot < a.num_slots;
-    if (store_kv) {
-      const int64_t page = slot < 0x7FFFFFFF ? (int64_t)div_by((uint32_t)slot, p.by_page) : slot / a.page_size;
-      const int64_t off = slot - page * a.page_size;
-      kdst = page * a.k_page_stride + off * a.k_row_stride;
-      vdst = page * a.v_page_stride + off * a.v_row_stride;
-    }
-  }
-  const int nk = a.q_heads + a.kv_heads;
-  const int heads = nk + (a.slot_map ? a.kv_heads : 0);
-#pragma unroll 4
-  for (int h = grp; h < heads; h += p.groups) {
+  for (int i = 0; i < ITEMS; ++i) {
+    const uint32_t idx = threadIdx.x + i * THREADS;
+    const uint32_t th = div_by(idx, p.by_units);
+    const int u = (int)(idx - th * p.units), tl = (int)div_by(th, p.by_heads), h = h0 + (int)(th - tl * p.heads);
+    dst[i] = nullptr;
+    if (tl >= toks || h >= h0 + heads) continue;
+    const int64_t tok = tok0 + tl;
+    const bool turn = u < p.turn_units;
+    // turned units hold VEC pairs; a copied unit is the one piece at rot + VEC c
+    const int o = !turn ? a.rot + VEC * (u - p.turn_units) : a.adjacent ? 2 * VEC * u : VEC * u;
+    first[i] = turn && h < nk ? tl * half + u * VEC : -1;
     const T* src;
-    T* dst;
+    T* to;
     if (h < a.q_heads) {
       src = (const T*)a.q + tok * a.q_stride + h * a.q_head_stride;
-      dst = (T*)a.q_out + (tok * a.q_heads + h) * a.d;
-    } else if (h < nk) {
-      const int kh = h - a.q_heads;
-      if (!store_kv) continue;
-      src = (const T*)a.k + tok * a.k_stride + kh * a.k_head_stride;
-      dst = a.slot_map ? (T*)a.k_cache + kdst + kh * a.k_cache_head_stride
-                       : (T*)a.k_out + (tok * a.kv_heads + kh) * a.d;
+      to = (T*)a.q_out + (tok * a.q_heads + h) * a.d;
     } else {
-      const int vh = h - nk;
-      if (!store_kv) continue;
-      src = (const T*)a.v + tok * a.v_stride + vh * a.v_head_stride;
-      dst = (T*)a.v_cache + vdst + vh * a.v_cache_head_stride;
-    }
-    P x = *(const P*)(src + o0), y;
-    if (turn) {
-      y = *(const P*)(src + o1);
-      if (h < nk) {
-        float e[2 * VEC];  // in pair order for adjacent pairs, else the first members then the second
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) e[i] = to_f(x.v[i]), e[VEC + i] = to_f(y.v[i]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int j0 = a.adjacent ? 2 * i : i, j1 = a.adjacent ? 2 * i + 1 : VEC + i;
-          const float f = e[j0], g = e[j1];
-          e[j0] = fmaf(f, c[i], -(g * s[i]));
-          e[j1] = fmaf(g, c[i], f * s[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x.v[i] = from_f<T>(e[i]), y.v[i] = from_f<T>(e[VEC + i]);
+      const bool key = h < nk;
+      const int kh = key ? h - a.q_heads : h - nk;
+      src = key ? (const T*)a.k + tok * a.k_stride + kh * a.k_head_stride
+                : (const T*)a.v + tok * a.v_stride + kh * a.v_head_stride;
+      if (a.slot_map) {
+        const int64_t slot = a.slot_map[tok];
+        if (slot < 0 || slot >= a.num_slots) continue;
+        const int64_t page = slot < 0x7FFFFFFF ? (int64_t)div_by((uint32_t)slot, p.by_page) : slot / a.page_size;
+        const int64_t off = slot - page * a.page_size;
+        to = key ? (T*)a.k_cache + page * a.k_page_stride + off * a.k_row_stride + kh * a.k_cache_head_stride
+                 : (T*)a.v_cache + page * a.v_page_stride + off * a.v_row_stride + kh * a.v_cache_head_stride;
+      } else {
+        to = (T*)a.k_out + (tok * a.kv_heads + kh) * a.d;
       }
-      *(P*)(dst + o1) = y;
     }
-    *(P*)(dst + o0) = x;
+    dst[i] = to + o;
+    x[i] = *(const P*)(src + o);
+    if (turn) y[i] = *(const P*)(src + o + apart), pairs |= 1u << i;
   }
+
+  for (uint32_t e = threadIdx.x; e < (uint32_t)(toks * half); e += THREADS) {
+    const int tl = (int)div_by(e, p.by_half), f = (int)(e - tl * half);
+    const int ax = a.axes ? min(max(a.axes[f], 0), a.num_axes - 1) : 0;
+    cs[e] = cos_sin(a.positions[ax * a.axis_stride + tok0 + tl], a.inv_freq[f], a.inverse);
+  }
+  __syncthreads();
+
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    if (!dst[i]) continue;
+    keep_packed(x[i]), keep_packed(y[i]);
+    if (first[i] >= 0) {
+      float e[2 * VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) e[j] = to_f(x[i].v[j]), e[VEC + j] = to_f(y[i].v[j]);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float2 t = cs[first[i] + j];
+        if (a.adjacent) {
+          const float f = e[2 * j], g = e[2 * j + 1];
+          e[2 * j] = fmaf(f, t.x, -(g * t.y)), e[2 * j + 1] = fmaf(g, t.x, f * t.y);
+        } else {
+          const float f = e[j], g = e[VEC + j];
+          e[j] = fmaf(f, t.x, -(g * t.y)), e[VEC + j] = fmaf(g, t.x, f * t.y);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[i].v[j] = from_f<T>(e[j]), y[i].v[j] = from_f<T>(e[VEC + j]);
+    }
+    *(P*)dst[i] = x[i];
+    if ((pairs >> i) & 1) *(P*)(dst[i] + apart) = y[i];
+  }
+}
+
+template <typename T, int VEC, int ITEMS>
+int launch_items(const ea_rope_t& a, Plan p, cudaStream_t st) {
+  const int room = THREADS * ITEMS;
+  p.heads = min(p.all_heads, room / p.units);
+  p.head_blocks = (p.all_heads + p.heads - 1) / p.heads;
+  p.tokens = p.head_blocks > 1 ? 1 : max(1, room / (p.units * p.all_heads));
+  while (p.tokens > 1 && p.tokens * (a.rot / 2) > 4096) p.tokens >>= 1;  // 32 KB of cos / sin
+  p.by_heads = fast_div((uint32_t)p.heads);
+  p.by_head_blocks = fast_div((uint32_t)p.head_blocks);
+  const int64_t blocks = (a.tokens + p.tokens - 1) / p.tokens * p.head_blocks;
+  if (blocks >= (1ll << 31)) return fail(-1, "rope: too many tokens");
+  rope_kernel<T, VEC, ITEMS><<<(unsigned)blocks, THREADS, sizeof(float2) * p.tokens * (a.rot / 2), st>>>(a, p);
+  return cuda_rc(cudaGetLastError());
 }
 
 template <typename T, int VEC>
@@ -126,20 +166,14 @@ int launch(const ea_rope_t& a, cudaStream_t st) {
   Plan p;
   p.turn_units = a.rot / 2 / VEC;
   p.units = p.turn_units + (a.d - a.rot) / VEC;
-  const int heads = a.q_heads + a.kv_heads * (a.slot_map ? 2 : 1);
-  // Heads a thread: 8 where there are tokens enough to fill the GPU four times over, fewer otherwise.
-  const int64_t want = (int64_t)sm_count() * 2048 * 4;
-  int per = 8;
-  while (per > 1 && a.tokens * p.units * ((heads + per - 1) / per) < want) per >>= 1;
-  p.groups = (heads + per - 1) / per;
+  p.all_heads = a.q_heads + a.kv_heads * (a.slot_map ? 2 : 1);
   p.by_units = fast_div((uint32_t)p.units);
-  p.by_groups = fast_div((uint32_t)p.groups);
-  p.by_page = fast_div((uint32_t)(a.page_size > 0 ? a.page_size : 1));
-  const int64_t items = a.tokens * p.units * p.groups;
-  const int64_t blocks = (items + THREADS - 1) / THREADS;
-  if (blocks > 0x7FFFFFFF) return fail(-1, "rope: too many tokens");
-  rope_kernel<T, VEC><<<(unsigned)blocks, THREADS, 0, st>>>(a, p);
-  return cuda_rc(cudaGetLastError());
+  p.by_half = fast_div((uint32_t)max(1, a.rot / 2));
+  p.by_page = fast_div((uint32_t)max(1, a.page_size));
+  // four pieces a thread keep enough bytes in flight; one where that would leave SMs without a block
+  const int64_t items = a.tokens * p.units * p.all_heads;
+  if (items > 4 * (int64_t)THREADS * 2 * sm_count() || p.units > THREADS) return launch_items<T, VEC, 4>(a, p, st);
+  return launch_items<T, VEC, 1>(a, p, st);
 }
 
 template <typename T>
@@ -167,7 +201,7 @@ extern "C" int ea_rope_cuda(const ea_rope_t* a, void* stream) {
   if (!a || a->tokens < 0 || a->q_heads < 0 || a->kv_heads < 0 || a->d <= 0 || a->rot < 0 || a->rot > a->d ||
       a->rot % 2 != 0 || a->num_axes < 1)
     return fail(-1, "rope: negative size, or rot odd or above d");
-  if (a->d > 8192 || a->q_heads > 65536 || a->kv_heads > 65536) return fail(-9, "rope: d above 8192 or above 65536 heads");
+  if (a->d > 1024 || a->q_heads > 65536 || a->kv_heads > 65536) return fail(-9, "rope: d above 1024 or above 65536 heads");
   if (a->tokens == 0 || a->q_heads + a->kv_heads == 0) return 0;
   if ((a->rot && (!a->positions || !a->inv_freq)) || (a->q_heads && (!a->q || !a->q_out)) || (a->kv_heads && !a->k))
     return fail(-1, "rope: a required pointer is NULL");

@@ -24,9 +24,9 @@ constexpr int ROWS = 16, WARPS = 4, KT = 16 * WARPS, THREADS = 32 * WARPS, STAGE
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// 16 bytes, or zeros where `ok` is false
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+// 16 bytes: `bytes` (16 or 0) from src, the rest zeros
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -63,18 +63,28 @@ __device__ __forceinline__ void mma<__half>(float* c, const uint32_t* a, uint32_
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack(__nv_bfloat16 x, __nv_bfloat16 y) {
-  return (uint32_t)__bfloat16_as_ushort(x) | (uint32_t)__bfloat16_as_ushort(y) << 16;
-}
-__device__ __forceinline__ uint32_t pack(__half x, __half y) {
-  return (uint32_t)__half_as_ushort(x) | (uint32_t)__half_as_ushort(y) << 16;
-}
 // two weights as their roundings and the roundings of what is left
 template <typename T>
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const T hx = from_f<T>(x), hy = from_f<T>(y);
-  hi = pack(hx, hy);
-  lo = pack(from_f<T>(x - to_f(hx)), from_f<T>(y - to_f(hy)));
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo);
+template <>
+__device__ __forceinline__ void split2<__nv_bfloat16>(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  hi = *(const uint32_t*)&h;
+  const __nv_bfloat162 r = __floats2bfloat162_rn(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
+  lo = *(const uint32_t*)&r;
+}
+template <>
+__device__ __forceinline__ void split2<__half>(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  hi = *(const uint32_t*)&h;
+  const float2 f = __half22float2(h);
+  const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+  lo = *(const uint32_t*)&r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // the two 16-bit numbers with infinities and NaN replaced by zeros
 template <typename T>
@@ -84,24 +94,13 @@ __device__ __forceinline__ uint32_t finite2(uint32_t v) {
   if ((v & EXP << 16) == EXP << 16) v &= 0xFFFFu;
   return v;
 }
-// whether four pairs of numbers hold an infinity or NaN: x * 0 summed up is 0 unless one does
-template <typename T>
-__device__ __forceinline__ bool not_finite(const uint32_t* f) {
-  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-  const uint32_t zero = 0;
-  T2 z = *(const T2*)&zero;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) z = __hfma2(*(const T2*)&f[e], *(const T2*)&zero, z);
-  return (*(const uint32_t*)&z & 0x7FFF7FFFu) != 0;
-}
-
 template <int DP>
 struct Smem {
   static constexpr int ROW_BYTES = DP * 2;
   static constexpr int SLICE = 16 * ROW_BYTES;                    // K or V of 16 keys
   static constexpr int STAGE = 2 * SLICE;                         // one warp's
-  static constexpr int POOL = WARPS * STAGES * STAGE;             // also the join's scratch
-  static_assert(POOL >= WARPS * ROWS * DP * 4, "the join fits into the stages");
+  static constexpr int POOL = WARPS * STAGES * STAGE + 256;       // aligned to 256 bytes; also the join's scratch
+  static_assert(POOL - 256 >= WARPS * ROWS * DP * 4, "the join fits into the stages");
 };
 
 template <int DP>
@@ -127,17 +126,10 @@ __device__ __forceinline__ void load_slice(const Args& a, const Item& it, int ke
 #pragma unroll
     for (int c = c0; c < PIECES; c += LANES_PER_ROW) {
       const bool in = ok && c * 8 < a.t.d;
-      cp16(stage + swz<DP>(r, c), in ? ks + c * 8 : (const T*)a.t.k_cache, in);
-      cp16(stage + Smem<DP>::SLICE + swz<DP>(r, c), in ? vs + c * 8 : (const T*)a.t.v_cache, in);
+      cp16(stage + swz<DP>(r, c), in ? ks + c * 8 : (const T*)a.t.k_cache, in ? 16 : 0);
+      cp16(stage + Smem<DP>::SLICE + swz<DP>(r, c), in ? vs + c * 8 : (const T*)a.t.v_cache, in ? 16 : 0);
     }
   }
-}
-
-__device__ __forceinline__ int page_of(const Args& a, const Item& it, int key0, int lane) {
-  const int key = key0 + (lane & 15);
-  if (key >= it.len) return -1;
-  const int p = a.t.page_table[it.b * a.t.table_stride + div_by((uint32_t)key, a.by_page)];
-  return p >= 0 && p < a.t.num_pages ? p : -1;
 }
 
 // Whether query row R of the item (token i of the step) sees key `key`.
@@ -153,8 +145,9 @@ __device__ __forceinline__ bool sees(const Args& a, const Item& it, int i, int k
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
   using S = Smem<DP>;
-  extern __shared__ __align__(128) uint8_t pool[];
-  uint32_t* sums = (uint32_t*)(pool + S::POOL);
+  extern __shared__ uint8_t raw[];
+  uint8_t* pool = (uint8_t*)(((uintptr_t)raw + 255) & ~(uintptr_t)255);
+  uint32_t* sums = (uint32_t*)(raw + S::POOL);
   __shared__ uint64_t scratch[32];
   __shared__ float join_m[WARPS][ROWS], join_l[WARPS][ROWS];
   Schedule<ROWS, KT> sch;
@@ -164,6 +157,17 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
   uint32_t pos = sch.share(blockIdx.x);
   const uint32_t end = sch.share(blockIdx.x + 1);
   const float alpha = a.t.alpha;
+  const bool in_page = a.t.page_size % 16 == 0;  // a slice lies in one page
+
+  // copies of a whole slice from one page: this lane's piece of rows lane / LPR, + RPI, ..; lanes past d fill in zeros
+  constexpr int LPR = DP / 8 < 8 ? DP / 8 : 8, RPI = 32 / LPR;
+  const int c0 = lane % LPR;
+  const int bytes0 = c0 * 8 < a.t.d ? 16 : 0, bytes1 = (c0 + 8) * 8 < a.t.d ? 16 : 0;
+  const int64_t k_lane = (lane / LPR) * a.t.k_row_stride + (bytes0 ? c0 * 8 : 0);
+  const int64_t v_lane = (lane / LPR) * a.t.v_row_stride + (bytes0 ? c0 * 8 : 0);
+  // fragment addresses inside a slice; a step of 16 channels flips address bits 5 and up
+  const uint32_t k_frag = ((lane & 7) + ((lane >> 4) << 3)) * S::ROW_BYTES + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  const uint32_t v_frag = S::SLICE + (lane & 15) * S::ROW_BYTES + (((lane >> 4) ^ (lane & 7)) << 4);
 
   while (pos < end) {
     const Item it = sch.item(a, pos, end);
@@ -190,143 +194,173 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
           qf[ks][half + 2 * p] = c < a.t.d ? *(const uint32_t*)(q + c) : 0u;
         }
     }
-    float o[DP / 8][4];
-#pragma unroll
-    for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-
     const int n = it.kt1 - it.kt0;
     const int key_w = it.kt0 * KT + warp * 16;
-    // pages one slice ahead of their copies
-    int page = page_of(a, it, key_w, lane);
-    uint32_t seen_pages[STAGES];  // which keys of a stage's slice have a page
+    const T* k_head = (const T*)a.t.k_cache + it.h * a.t.k_head_stride + k_lane;
+    const T* v_head = (const T*)a.t.v_cache + it.h * a.t.v_head_stride + v_lane;
+    const int32_t* pages = a.t.page_table + it.b * a.t.table_stride;
+    // the page of a slice, fetched one slice ahead of its copies: the slice's (in_page) or the lane's key's
+    const auto page_of = [&](int key0) {
+      const int key = in_page ? key0 : key0 + (lane & 15);
+      if (key >= it.len) return -1;
+      const int p = pages[div_by((uint32_t)key, a.by_page)];
+      return p >= 0 && p < a.t.num_pages ? p : -1;
+    };
+    // issues a slice's copies; which of its keys exist
+    const auto load = [&](int key0, int page, uint32_t stage) -> uint32_t {
+      if (in_page && page >= 0 && key0 + 16 <= it.len) {
+        const int off = key0 - (int)div_by((uint32_t)key0, a.by_page) * a.t.page_size;
+        const T* ks = k_head + page * a.t.k_page_stride + off * a.t.k_row_stride;
+        const T* vs = v_head + page * a.t.v_page_stride + off * a.t.v_row_stride;
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-      if (s < n) load_slice<T, DP>(a, it, key_w + s * KT, page, base + s * S::STAGE, lane);
-      seen_pages[s] = __ballot_sync(0xffffffffu, page >= 0);
-      cp_commit();
-      page = page_of(a, it, key_w + (s + 1) * KT, lane);
-    }
-    seen_pages[STAGES - 1] = 0;
-    int stage = 0;
-    for (int t = 0; t < n; ++t) {
-      cp_wait<STAGES - 2>();
-      __syncwarp();
-      {
-        const int nt = t + STAGES - 1;
-        int ns = stage + STAGES - 1;
-        if (ns >= STAGES) ns -= STAGES;
-        if (nt < n) load_slice<T, DP>(a, it, key_w + nt * KT, page, base + ns * S::STAGE, lane);
-        const uint32_t bl = __ballot_sync(0xffffffffu, page >= 0);
-#pragma unroll
-        for (int s = 0; s < STAGES; ++s)
-          if (s == ns) seen_pages[s] = bl;
-        cp_commit();
-        page = page_of(a, it, key_w + (nt + 1) * KT, lane);
+        for (int r0 = 0; r0 < 16; r0 += RPI) {
+          const uint32_t at = stage + swz<DP>(r0 + lane / LPR, c0);
+          cp16(at, ks, bytes0);
+          cp16(at + S::SLICE, vs, bytes0);
+          if (DP == 128) {
+            cp16(at ^ 128, ks + 64, bytes1);  // piece c0 + 8
+            cp16((at ^ 128) + S::SLICE, vs + 64, bytes1);
+          }
+          ks += RPI * a.t.k_row_stride;
+          vs += RPI * a.t.v_row_stride;
+        }
+        return 0xFFFFu;
       }
-      uint32_t okm = 0;
-#pragma unroll
-      for (int s = 0; s < STAGES; ++s)
-        if (s == stage) okm = seen_pages[s];
-      const uint32_t kb = base + stage * S::STAGE, vb = kb + S::SLICE;
-      const int key0 = key_w + t * KT;
+      if (in_page && key0 + (lane & 15) >= it.len) page = -1;
+      load_slice<T, DP>(a, it, key0, page, stage, lane);
+      return __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
+    };
 
-      // scores: s[nt][..] rows lane / 4 (+ 8), keys nt * 8 + 2 (lane % 4) (+ 1)
-      float s[2][4];
+    float o[DP / 8][4], m[2], l[2];
+    // The first pass takes the values as they are. An infinity or NaN among them may not meet the zero weight of a row
+    // that does not see its key, nor a weight's remainder: if any output is not finite, a second pass takes
+    // such values out of the product and adds them to the rows that see them one by one.
+    for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.0f;
+      for (int nn = 0; nn < DP / 8; ++nn)
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        if (ks * 16 < a.t.d) {
-          uint32_t f[4];
-          ldsm4(kb + swz<DP>((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), f);
-          mma<T>(s[0], qf[ks], f[0], f[1]);
-          mma<T>(s[1], qf[ks], f[2], f[3]);
-        }
+        for (int e = 0; e < 4; ++e) o[nn][e] = 0.0f;
+      m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.0f;
+      uint32_t exist[STAGES];  // of the slices under way, oldest first
+      int page = page_of(key_w);
+#pragma unroll
+      for (int s = 0; s < STAGES - 1; ++s) {
+        exist[s] = s < n ? load(key_w + s * KT, page, base + s * S::STAGE) : 0;
+        cp_commit();
+        page = page_of(key_w + (s + 1) * KT);
       }
-      const bool masked = key0 + 16 > ctx || (okm & 0xFFFFu) != 0xFFFFu;
-      float mx[2] = {-INFINITY, -INFINITY};
+      uint32_t cur = base, ahead = base + (STAGES - 1) * S::STAGE;
+      for (int t = 0; t < n; ++t) {
+        cp_wait<STAGES - 2>();
+        __syncwarp();
+        const int nt = t + STAGES - 1;
+        exist[STAGES - 1] = nt < n ? load(key_w + nt * KT, page, ahead) : 0;
+        cp_commit();
+        page = page_of(key_w + (nt + 1) * KT);
+        const int key0 = key_w + t * KT;
+        const uint32_t okm = exist[0];
+
+        // scores: s[nt][..] rows lane / 4 (+ 8), keys nt * 8 + 2 (lane % 4) (+ 1)
+        float s[2][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+        for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[nt][e] *= alpha;
-          if (masked) {
-            const int kk = nt * 8 + 2 * (lane & 3) + (e & 1);
-            if (!sees(a, it, tok[e >> 1], key0 + kk, (okm >> kk) & 1)) s[nt][e] = -INFINITY;
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          if (ks * 16 < a.t.d) {
+            uint32_t f[4];
+            ldsm4((cur + k_frag) ^ (ks * 32), f);
+            mma<T>(s[0], qf[ks], f[0], f[1]);
+            mma<T>(s[1], qf[ks], f[2], f[3]);
           }
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[nt][e]);
         }
-      float scale[2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
-        mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
-        const float mn = fmaxf(m[half], mx[half]);
-        const float ref = mn == -INFINITY ? 0.0f : mn;
-        scale[half] = exp2f(m[half] - ref);
-        m[half] = mn;
-        l[half] *= scale[half];
+        for (int nt2 = 0; nt2 < 2; ++nt2)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+          for (int e = 0; e < 4; ++e) s[nt2][e] *= alpha;
+        if (key0 + 16 > ctx || okm != 0xFFFFu) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            s[nt][2 * half + e] = exp2f(s[nt][2 * half + e] - ref);
-            l[half] += s[nt][2 * half + e];
-          }
-      }
-      if (__any_sync(0xffffffffu, scale[0] != 1.0f || scale[1] != 1.0f)) {
+          for (int nt2 = 0; nt2 < 2; ++nt2)
 #pragma unroll
-        for (int nn = 0; nn < DP / 8; ++nn)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nn][e] *= scale[e >> 1];
-      }
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-          split2<T>(s[nt][2 * half], s[nt][2 * half + 1], hi[nt * 2 + half], lo[nt * 2 + half]);
-      // an infinity or NaN among the values may not meet the zero weight of a row that does not see its key,
-      // nor a weight's remainder: such values leave the product and reach the rows that see them one by one
-      bool bad = false;
-#pragma unroll
-      for (int nn = 0; nn < DP / 16; ++nn) {
-        if (nn * 16 < a.t.d) {
-          uint32_t f[4];
-          ldsm4_t(vb + swz<DP>(lane & 15, nn * 2 + (lane >> 4)), f);
-          if (not_finite<T>(f)) {
-            bad = true;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = finite2<T>(f[e]);
-          }
-          mma<T>(o[2 * nn], hi, f[0], f[1]);
-          mma<T>(o[2 * nn + 1], hi, f[2], f[3]);
-          mma<T>(o[2 * nn], lo, f[0], f[1]);
-          mma<T>(o[2 * nn + 1], lo, f[2], f[3]);
+            for (int e = 0; e < 4; ++e) {
+              const int kk = nt2 * 8 + 2 * (lane & 3) + (e & 1);
+              if (!sees(a, it, tok[e >> 1], key0 + kk, (okm >> kk) & 1)) s[nt2][e] = -INFINITY;
+            }
         }
-      }
-      if (__any_sync(0xffffffffu, bad)) {
-        for (int kk = 0; kk < 16; ++kk) {
-          const bool see0 = sees(a, it, tok[0], key0 + kk, (okm >> kk) & 1), see1 = sees(a, it, tok[1], key0 + kk, (okm >> kk) & 1);
+        float scale[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float mx = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float mn = fmaxf(m[half], mx), ref = mn == -INFINITY ? 0.0f : mn;
+          scale[half] = ex2(m[half] - ref);
+          m[half] = mn;
+          l[half] *= scale[half];
+#pragma unroll
+          for (int nt2 = 0; nt2 < 2; ++nt2)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              s[nt2][2 * half + e] = ex2(s[nt2][2 * half + e] - ref);
+              l[half] += s[nt2][2 * half + e];
+            }
+        }
+        if (__any_sync(0xffffffffu, scale[0] != 1.0f || scale[1] != 1.0f)) {
 #pragma unroll
           for (int nn = 0; nn < DP / 8; ++nn)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int c = nn * 8 + 2 * (lane & 3) + e;
-              const float f = to_f(*(const T*)(pool + (vb - smem_addr(pool)) + swz<DP>(kk, c >> 3) + (c & 7) * 2));
-              if (isfinite(f)) continue;
-              if (see0) o[nn][e] += f;
-              if (see1) o[nn][2 + e] += f;
-            }
+            for (int e = 0; e < 4; ++e) o[nn][e] *= scale[e >> 1];
         }
-        __syncwarp();
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int nt2 = 0; nt2 < 2; ++nt2)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            split2<T>(s[nt2][2 * half], s[nt2][2 * half + 1], hi[nt2 * 2 + half], lo[nt2 * 2 + half]);
+#pragma unroll
+        for (int nn = 0; nn < DP / 16; ++nn) {
+          if (nn * 16 < a.t.d) {
+            uint32_t f[4];
+            ldsm4_t((cur + v_frag) ^ (nn * 32), f);
+            if (pass) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f[e] = finite2<T>(f[e]);
+            }
+            mma<T>(o[2 * nn], hi, f[0], f[1]);
+            mma<T>(o[2 * nn + 1], hi, f[2], f[3]);
+            mma<T>(o[2 * nn], lo, f[0], f[1]);
+            mma<T>(o[2 * nn + 1], lo, f[2], f[3]);
+          }
+        }
+        if (pass) {
+          for (int kk = 0; kk < 16; ++kk) {
+            const bool see0 = sees(a, it, tok[0], key0 + kk, (okm >> kk) & 1), see1 = sees(a, it, tok[1], key0 + kk, (okm >> kk) & 1);
+#pragma unroll
+            for (int nn = 0; nn < DP / 8; ++nn)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int c = nn * 8 + 2 * (lane & 3) + e;
+                const float f = to_f(*(const T*)(pool + (cur - smem_addr(pool)) + S::SLICE + swz<DP>(kk, c >> 3) + (c & 7) * 2));
+                if (isfinite(f)) continue;
+                if (see0) o[nn][e] += f;
+                if (see1) o[nn][2 + e] += f;
+              }
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i + 1 < STAGES; ++i) exist[i] = exist[i + 1];
+        cur = cur == base + (STAGES - 1) * S::STAGE ? base : cur + S::STAGE;
+        ahead = ahead == base + (STAGES - 1) * S::STAGE ? base : ahead + S::STAGE;
       }
-      if (++stage == STAGES) stage = 0;
+      cp_wait<0>();
+      __syncwarp();
+      float probe = 0.0f;
+#pragma unroll
+      for (int nn = 0; nn < DP / 8; ++nn)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) probe = fmaf(o[nn][e], 0.0f, probe);  // NaN if one is not finite
+      if (!__any_sync(0xffffffffu, probe != 0.0f)) break;
     }
-    cp_wait<0>();
 
     // join the warps
 #pragma unroll
@@ -382,7 +416,14 @@ template <typename T, int DP>
 int launch(Args& a, cudaStream_t st) {
   const size_t smem = Smem<DP>::POOL + 4 * (size_t)(a.t.batch + 1);
   const size_t csmem = 4 * (size_t)(a.t.batch + 1);
-  cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static bool ready[64];  // per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
+    e = cudaFuncSetAttribute(few_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Smem<DP>::POOL + 4 * (EA_TREE_MAX_SEQS + 1));
+    if (e == cudaSuccess && dev < 64) ready[dev] = true;
+  }
   if (e != cudaSuccess) return cuda_rc(e);
   few_rows_kernel<T, DP><<<a.workers, THREADS, smem, st>>>(a);
   e = cudaGetLastError();
