@@ -6,9 +6,11 @@
 // built from the row's history, path and bias list while the first logits are on their way:
 //   bits 0-19 how often the token was generated, bits 20-30 which bias entry it has first
 //   (EA_LOGITS_MAX_BIASES - entry, 0: none), bit 31 whether the prompt holds it.
-// The words are integers, so the order of the atomics cannot change them. The corrections walk over the same lists:
-// who swaps a token's nonzero word for zero corrects the token. So the dense part reads no table, and the cost of the
-// sparse part follows the lists' lengths. Rows without penalties and biases build no table.
+// The words are integers, so the order of the atomics cannot change them. Whoever finds a token's word zero puts the
+// token on a list, from which the corrections are then done with full warps (in place, lanes with and without a
+// token in their part of the history took turns: 80 us for 256 rows of 131072 tokens with 4096 history entries). So the
+// dense part reads no table, and the cost of the sparse part follows the lists' lengths. Rows without penalties
+// and biases build no table.
 #include "ea_serving.cuh"
 
 namespace ea {
@@ -17,6 +19,7 @@ namespace {
 
 constexpr int THREADS = 512;
 constexpr int UNROLL = 4;  // 16-byte pieces a thread has in flight
+constexpr int BATCH = 8;   // history entries of a thread at a time
 constexpr uint32_t COUNT = 0xFFFFFu, PROMPT = 0x80000000u;
 constexpr int CODE_SHIFT = 20;
 
@@ -54,7 +57,8 @@ __global__ void __launch_bounds__(THREADS, 2) logits_kernel(ea_process_logits_t 
   using P = Pack<T, VEC>;
   extern __shared__ uint4 table4[];
   uint32_t* table = (uint32_t*)table4;
-  __shared__ int dup;
+  uint16_t* list = (uint16_t*)(table + chunk);  // tokens with a nonzero word
+  __shared__ int dup, listed;
   const int tid = threadIdx.x;
   const int64_t row = div_by(blockIdx.x, by_chunks);
   const int part = (int)(blockIdx.x - row * chunks);
@@ -89,11 +93,43 @@ __global__ void __launch_bounds__(THREADS, 2) logits_kernel(ea_process_logits_t 
   int n_hist = 0, n_prompt = 0, n_path = 0;
   const int32_t *hist = nullptr, *path = nullptr;
   const uint32_t* seen = nullptr;
+  bool hist4 = false;
+  uint32_t tok[BATCH];  // places in the chunk of the thread's first history entries (>= span: elsewhere)
+  // entries first + 4 (512 j + tid) + 0 .. 3, j = 0, 1
+  const auto fetch = [&](int first) {
+#pragma unroll
+    for (int j = 0; j < BATCH / 4; ++j) {
+      const int i = first + 4 * (j * THREADS + tid);
+      int4 h = make_int4(-1, -1, -1, -1);
+      if (hist4 && i + 4 <= a.max_history) {
+        h = *(const int4*)(hist + i);
+      } else {
+        if (i < a.max_history) h.x = hist[i];
+        if (i + 1 < a.max_history) h.y = hist[i + 1];
+        if (i + 2 < a.max_history) h.z = hist[i + 2];
+        if (i + 3 < a.max_history) h.w = hist[i + 3];
+      }
+      tok[4 * j] = (uint32_t)h.x - lo, tok[4 * j + 1] = (uint32_t)h.y - lo;
+      tok[4 * j + 2] = (uint32_t)h.z - lo, tok[4 * j + 3] = (uint32_t)h.w - lo;
+    }
+  };
+  const auto entry = [&](int first, int e) { return first + 4 * ((e >> 2) * THREADS + tid) + (e & 3); };
+  // puts a token on the list if its word was zero before
+  const auto touch = [&](uint32_t t, uint32_t before) {
+    if (before) return;
+    const uint32_t together = __activemask(), below = together & ((1u << (tid & 31)) - 1);
+    int at = 0;
+    if (!below) at = atomicAdd(&listed, __popc(together));
+    at = __shfl_sync(together, at, __ffs(together) - 1);
+    list[at + __popc(below)] = (uint16_t)t;
+  };
   if (tabled) {
     if (counts && a.history) {
+      hist = a.history + (int64_t)b * a.history_stride;
+      hist4 = ((uintptr_t)hist & 15) == 0;
+      fetch(0);
       n_hist = min(max(a.history_lens[b], 0), a.max_history);
       n_prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), n_hist) : 0;
-      hist = a.history + (int64_t)b * a.history_stride;
     }
     if (counts && a.draft_tokens) {
       const int64_t q0 = a.q_start[b], q1 = min((int64_t)a.q_start[b + 1], a.rows);
@@ -106,20 +142,22 @@ __global__ void __launch_bounds__(THREADS, 2) logits_kernel(ea_process_logits_t 
     r.ids = a.bias_ids + (int64_t)b * a.num_biases;
     r.vals = a.bias_values + (int64_t)b * a.num_biases;
     for (int i = tid; i < (int)(span + 3) / 4; i += THREADS) table4[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) dup = 0;
+    if (tid == 0) dup = listed = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int i = tid; i < n_hist; i += THREADS) {
-      const uint32_t t = (uint32_t)hist[i] - lo;
-      if (t < span) {
-        if (i < n_prompt) atomicOr(table + t, PROMPT);
-        else atomicAdd(table + t, 1u);
+    for (int first = 0; first < n_hist; first += BATCH * THREADS) {
+      if (first) fetch(first);
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        const int i = entry(first, e);
+        if (tok[e] < span && i < n_hist) {
+          touch(tok[e], i < n_prompt ? atomicOr(table + tok[e], PROMPT) : atomicAdd(table + tok[e], 1u));
+        }
       }
     }
     for (int j = tid; j < n_path; j += THREADS) {
       if (seen && !((seen[j >> 5] >> (j & 31)) & 1)) continue;
       const uint32_t t = (uint32_t)path[j] - lo;
-      if (t < span) atomicAdd(table + t, 1u);
+      if (t < span) touch(t, atomicAdd(table + t, 1u));
     }
     __syncthreads();
     if (biased) {
@@ -129,6 +167,7 @@ __global__ void __launch_bounds__(THREADS, 2) logits_kernel(ea_process_logits_t 
           const uint32_t code = (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT;
           const uint32_t old = atomicMax(table + t, (table[t] & (PROMPT | COUNT)) | code);
           if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
+          touch(t, old);
         }
       }
     }
@@ -173,18 +212,12 @@ __global__ void __launch_bounds__(THREADS, 2) logits_kernel(ea_process_logits_t 
 
   __syncthreads();  // the chunk is written and the table complete
   r.dup = dup != 0;
-  const auto correct = [&](uint32_t t) {
-    if (t >= span || !table[t]) return;
-    const uint32_t w = atomicExch(table + t, 0u);
-    if (!w) return;
+  for (int i = tid; i < listed; i += THREADS) {
+    const uint32_t t = list[i];
     const int v = (int)(lo + t);
-    if (bits && !((bits[v >> 5] >> (v & 31)) & 1)) return;
-    dst[v] = from_f<T>(adjust(to_f(src[v]), w, v, r, a.num_biases));
-  };
-  for (int i = tid; i < n_hist; i += THREADS) correct((uint32_t)hist[i] - lo);
-  for (int j = tid; j < n_path; j += THREADS) correct((uint32_t)path[j] - lo);
-  if (biased)
-    for (int e = tid; e < a.num_biases; e += THREADS) correct((uint32_t)r.ids[e] - lo);
+    if (bits && !((bits[v >> 5] >> (v & 31)) & 1)) continue;
+    dst[v] = from_f<T>(adjust(to_f(src[v]), table[t], v, r, a.num_biases));
+  }
 }
 
 template <typename T, int VEC>
@@ -193,10 +226,17 @@ int launch(const ea_process_logits_t& a, cudaStream_t st) {
   int chunk = 16384;
   while (chunk > 2048 && a.rows * ((a.vocab + chunk - 1) / chunk) < 2 * sm_count()) chunk >>= 1;
   const int chunks = (int)(((int64_t)a.vocab + VEC - 1 + chunk - 1) / chunk);
+  chunk = (int)((((int64_t)a.vocab + VEC - 1 + chunks - 1) / chunks + 15) & ~15ll);  // equal chunks
   const int64_t blocks = a.rows * chunks;
   if (blocks > 0x7FFFFFFF) return fail(-1, "process_logits: too many rows");
-  const size_t smem = (size_t)chunk * 4;
-  const cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+  const size_t smem = (size_t)chunk * 6;
+  static bool ready[64];  // per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
+    e = cudaFuncSetAttribute(logits_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 6 * 16400);
+    if (e == cudaSuccess && dev < 64) ready[dev] = true;
+  }
   if (e != cudaSuccess) return cuda_rc(e);
   logits_kernel<T, VEC><<<(unsigned)blocks, THREADS, smem, st>>>(a, chunk, fast_div((uint32_t)chunks), chunks);
   return cuda_rc(cudaGetLastError());

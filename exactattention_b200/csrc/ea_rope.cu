@@ -2,21 +2,20 @@
 //   (x, y) -> (x c - y s, y c + x s),
 // optionally with the write of the turned keys and of the values into paged cache rows.
 //
-// Bound by HBM: every element is read once and written once. A block takes a few tokens with some or all of their
-// heads; its threads first load their pieces (two 16-byte pieces of a head hold VEC pairs), then compute the
-// cos / sin of the block's tokens into shared memory, one pair of them per (token, frequency), while the loads are
-// under way, and turn and store the pieces. The angle is reduced in 32 bits without loss: turns = position * f with
-// f = inv_freq / 2 pi as a sum of two numbers, the product's rounding error recovered by an FMA, the nearest integer
-// taken off the large part (exact); what is left of 2^-47 relative error is far below a 32-bit result's rounding.
-// sincospif then sees an argument in [-1, 1] whatever the position. Positions of 2^24 and more, which binary32 does
-// not hold, go through binary64.
+// Bound by HBM: every element is read once and written once. A thread owns one piece (two 16-byte parts of a head
+// that hold VEC pairs) of one token and takes it from up to four heads: it loads all of them, the block computes the
+// cos / sin of its tokens into shared memory while the loads are under way, once per (token, frequency), and the
+// thread turns and stores its pieces with them. The angle is reduced in 32 bits without loss: turns = position * f
+// with f = inv_freq / 2 pi as a sum of two numbers, the product's rounding error recovered by an FMA, the nearest
+// integer taken off the large part (exact); what is left of 2^-47 relative error is far below a 32-bit result's
+// rounding. sincospif then sees an argument in [-1, 1] whatever the position. Positions of 2^24 and more, which
+// binary32 does not hold, go through binary64.
 #include "ea_serving.cuh"
 
 namespace ea {
 namespace serving {
 namespace {
 
-constexpr int THREADS = 256;
 constexpr double INV_2PI = 0.15915494309189533577;  // 1 / (2 pi)
 
 template <typename T, int VEC>
@@ -35,10 +34,10 @@ __device__ __forceinline__ void keep_packed(Pack<T, VEC>& p) {
 }
 
 struct Plan {
-  int units, turn_units;        // pieces of a head: those that are turned first, then copied ones
-  int tokens, heads, head_blocks;  // of a block; blocks a token group
-  int all_heads;
-  FastDiv by_units, by_heads, by_half, by_page, by_head_blocks;
+  int units, turn_units;  // pieces of a head: those that are turned first, then copied ones
+  int tokens, lanes;      // of a block: tokens, and heads that are worked on at the same time
+  int head_blocks, all_heads;
+  FastDiv by_units, by_lanes, by_half, by_page, by_head_blocks;
 };
 
 __device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
@@ -59,105 +58,113 @@ __device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
   return cs;
 }
 
-template <typename T, int VEC, int ITEMS>
-__global__ void __launch_bounds__(THREADS, 3) rope_kernel(ea_rope_t a, Plan p) {
+template <typename T, int VEC, int ITEMS, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 3 : 1) rope_kernel(ea_rope_t a, Plan p) {
   using P = Pack<T, VEC>;
   extern __shared__ float2 cs[];  // (tokens, rot / 2)
   const uint32_t group = div_by(blockIdx.x, p.by_head_blocks);
   const int64_t tok0 = (int64_t)group * p.tokens;
-  const int h0 = (int)(blockIdx.x - group * p.head_blocks) * p.heads;
   const int nk = a.q_heads + a.kv_heads, half = a.rot / 2;
-  const int toks = (int)min((int64_t)p.tokens, a.tokens - tok0), heads = min(p.heads, p.all_heads - h0);
+  const int toks = (int)min((int64_t)p.tokens, a.tokens - tok0);
+  const uint32_t th = div_by(threadIdx.x, p.by_units);
+  const int u = (int)(threadIdx.x - th * p.units), tl = (int)div_by(th, p.by_lanes);
+  const int h0 = (int)(blockIdx.x - group * p.head_blocks) * p.lanes * ITEMS + (int)(th - tl * p.lanes);
+  const int64_t tok = tok0 + tl;
+  const bool turn = u < p.turn_units, live = tl < toks;
+  // turned units hold VEC pairs; a copied unit is the one piece at rot + VEC c
+  const int o = !turn ? a.rot + VEC * (u - p.turn_units) : a.adjacent ? 2 * VEC * u : VEC * u;
+  const int apart = a.adjacent ? VEC : half;  // from the first part of a piece to the second
 
+  int64_t k_row = 0, v_row = 0;
+  bool stored = true;  // the token's key and value have a place
+  if (a.slot_map && live) {
+    const int64_t slot = a.slot_map[tok];
+    stored = slot >= 0 && slot < a.num_slots;
+    const int64_t page = slot < 0x7FFFFFFF ? (int64_t)div_by((uint32_t)slot, p.by_page) : slot / a.page_size;
+    const int64_t off = slot - page * a.page_size;
+    k_row = page * a.k_page_stride + off * a.k_row_stride;
+    v_row = page * a.v_page_stride + off * a.v_row_stride;
+  }
   P x[ITEMS], y[ITEMS];
-  T* dst[ITEMS];       // of the first piece; nullptr: nothing to do
-  int first[ITEMS];    // of the piece's cos / sin; -1: copied
-  uint32_t pairs = 0;  // bit i: item i has a second piece
-  const int apart = a.adjacent ? VEC : half;  // from the first piece
+  T* dst[ITEMS];  // nullptr: nothing to do
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const uint32_t idx = threadIdx.x + i * THREADS;
-    const uint32_t th = div_by(idx, p.by_units);
-    const int u = (int)(idx - th * p.units), tl = (int)div_by(th, p.by_heads), h = h0 + (int)(th - tl * p.heads);
+    const int h = h0 + i * p.lanes;
     dst[i] = nullptr;
-    if (tl >= toks || h >= h0 + heads) continue;
-    const int64_t tok = tok0 + tl;
-    const bool turn = u < p.turn_units;
-    // turned units hold VEC pairs; a copied unit is the one piece at rot + VEC c
-    const int o = !turn ? a.rot + VEC * (u - p.turn_units) : a.adjacent ? 2 * VEC * u : VEC * u;
-    first[i] = turn && h < nk ? tl * half + u * VEC : -1;
+    if (!live || h >= p.all_heads || (h >= a.q_heads && !stored)) continue;
     const T* src;
-    T* to;
     if (h < a.q_heads) {
       src = (const T*)a.q + tok * a.q_stride + h * a.q_head_stride;
-      to = (T*)a.q_out + (tok * a.q_heads + h) * a.d;
+      dst[i] = (T*)a.q_out + (tok * a.q_heads + h) * a.d + o;
+    } else if (h < nk) {
+      const int kh = h - a.q_heads;
+      src = (const T*)a.k + tok * a.k_stride + kh * a.k_head_stride;
+      dst[i] = (a.slot_map ? (T*)a.k_cache + k_row + kh * a.k_cache_head_stride
+                           : (T*)a.k_out + (tok * a.kv_heads + kh) * a.d) + o;
     } else {
-      const bool key = h < nk;
-      const int kh = key ? h - a.q_heads : h - nk;
-      src = key ? (const T*)a.k + tok * a.k_stride + kh * a.k_head_stride
-                : (const T*)a.v + tok * a.v_stride + kh * a.v_head_stride;
-      if (a.slot_map) {
-        const int64_t slot = a.slot_map[tok];
-        if (slot < 0 || slot >= a.num_slots) continue;
-        const int64_t page = slot < 0x7FFFFFFF ? (int64_t)div_by((uint32_t)slot, p.by_page) : slot / a.page_size;
-        const int64_t off = slot - page * a.page_size;
-        to = key ? (T*)a.k_cache + page * a.k_page_stride + off * a.k_row_stride + kh * a.k_cache_head_stride
-                 : (T*)a.v_cache + page * a.v_page_stride + off * a.v_row_stride + kh * a.v_cache_head_stride;
-      } else {
-        to = (T*)a.k_out + (tok * a.kv_heads + kh) * a.d;
-      }
+      src = (const T*)a.v + tok * a.v_stride + (h - nk) * a.v_head_stride;
+      dst[i] = (T*)a.v_cache + v_row + (h - nk) * a.v_cache_head_stride + o;
     }
-    dst[i] = to + o;
     x[i] = *(const P*)(src + o);
-    if (turn) y[i] = *(const P*)(src + o + apart), pairs |= 1u << i;
+    if (turn) y[i] = *(const P*)(src + o + apart);
   }
 
   for (uint32_t e = threadIdx.x; e < (uint32_t)(toks * half); e += THREADS) {
-    const int tl = (int)div_by(e, p.by_half), f = (int)(e - tl * half);
+    const int t = (int)div_by(e, p.by_half), f = (int)(e - t * half);
     const int ax = a.axes ? min(max(a.axes[f], 0), a.num_axes - 1) : 0;
-    cs[e] = cos_sin(a.positions[ax * a.axis_stride + tok0 + tl], a.inv_freq[f], a.inverse);
+    cs[e] = cos_sin(a.positions[ax * a.axis_stride + tok0 + t], a.inv_freq[f], a.inverse);
   }
   __syncthreads();
+  float c[VEC], s[VEC];
+  if (turn && live) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float2 t = cs[tl * half + u * VEC + j];
+      c[j] = t.x, s[j] = t.y;
+    }
+  }
 
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     if (!dst[i]) continue;
     keep_packed(x[i]), keep_packed(y[i]);
-    if (first[i] >= 0) {
+    if (turn && h0 + i * p.lanes < nk) {
       float e[2 * VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) e[j] = to_f(x[i].v[j]), e[VEC + j] = to_f(y[i].v[j]);
+      if (a.adjacent) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float2 t = cs[first[i] + j];
-        if (a.adjacent) {
+        for (int j = 0; j < VEC; ++j) {
           const float f = e[2 * j], g = e[2 * j + 1];
-          e[2 * j] = fmaf(f, t.x, -(g * t.y)), e[2 * j + 1] = fmaf(g, t.x, f * t.y);
-        } else {
+          e[2 * j] = fmaf(f, c[j], -(g * s[j])), e[2 * j + 1] = fmaf(g, c[j], f * s[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
           const float f = e[j], g = e[VEC + j];
-          e[j] = fmaf(f, t.x, -(g * t.y)), e[VEC + j] = fmaf(g, t.x, f * t.y);
+          e[j] = fmaf(f, c[j], -(g * s[j])), e[VEC + j] = fmaf(g, c[j], f * s[j]);
         }
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[i].v[j] = from_f<T>(e[j]), y[i].v[j] = from_f<T>(e[VEC + j]);
     }
     *(P*)dst[i] = x[i];
-    if ((pairs >> i) & 1) *(P*)(dst[i] + apart) = y[i];
+    if (turn) *(P*)(dst[i] + apart) = y[i];
   }
 }
 
-template <typename T, int VEC, int ITEMS>
+template <typename T, int VEC, int ITEMS, int THREADS>
 int launch_items(const ea_rope_t& a, Plan p, cudaStream_t st) {
-  const int room = THREADS * ITEMS;
-  p.heads = min(p.all_heads, room / p.units);
-  p.head_blocks = (p.all_heads + p.heads - 1) / p.heads;
-  p.tokens = p.head_blocks > 1 ? 1 : max(1, room / (p.units * p.all_heads));
-  while (p.tokens > 1 && p.tokens * (a.rot / 2) > 4096) p.tokens >>= 1;  // 32 KB of cos / sin
-  p.by_heads = fast_div((uint32_t)p.heads);
+  const int want = (p.all_heads + ITEMS - 1) / ITEMS;  // lanes for all heads in one block
+  p.lanes = min(want, THREADS / p.units);
+  p.head_blocks = (p.all_heads + p.lanes * ITEMS - 1) / (p.lanes * ITEMS);
+  p.tokens = p.head_blocks > 1 ? 1 : max(1, THREADS / (p.units * p.lanes));
+  p.by_lanes = fast_div((uint32_t)p.lanes);
   p.by_head_blocks = fast_div((uint32_t)p.head_blocks);
   const int64_t blocks = (a.tokens + p.tokens - 1) / p.tokens * p.head_blocks;
   if (blocks >= (1ll << 31)) return fail(-1, "rope: too many tokens");
-  rope_kernel<T, VEC, ITEMS><<<(unsigned)blocks, THREADS, sizeof(float2) * p.tokens * (a.rot / 2), st>>>(a, p);
+  // at most THREADS / units tokens of rot / 2 <= units * VEC pairs: 8 KB per VEC
+  rope_kernel<T, VEC, ITEMS, THREADS><<<(unsigned)blocks, THREADS, sizeof(float2) * p.tokens * (a.rot / 2), st>>>(a, p);
   return cuda_rc(cudaGetLastError());
 }
 
@@ -170,10 +177,14 @@ int launch(const ea_rope_t& a, cudaStream_t st) {
   p.by_units = fast_div((uint32_t)p.units);
   p.by_half = fast_div((uint32_t)max(1, a.rot / 2));
   p.by_page = fast_div((uint32_t)max(1, a.page_size));
-  // four pieces a thread keep enough bytes in flight; one where that would leave SMs without a block
-  const int64_t items = a.tokens * p.units * p.all_heads;
-  if (items > 4 * (int64_t)THREADS * 2 * sm_count() || p.units > THREADS) return launch_items<T, VEC, 4>(a, p, st);
-  return launch_items<T, VEC, 1>(a, p, st);
+  if constexpr (VEC == 1) {
+    return launch_items<T, 1, 1, 1024>(a, p, st);  // up to 1024 single pairs a head
+  } else {
+    // four pieces a thread keep enough bytes in flight; one where that would leave SMs without a block
+    const int64_t items = a.tokens * p.units * p.all_heads;
+    if (items > 4 * 256 * 2 * (int64_t)sm_count()) return launch_items<T, VEC, 4, 256>(a, p, st);
+    return launch_items<T, VEC, 1, 256>(a, p, st);
+  }
 }
 
 template <typename T>
