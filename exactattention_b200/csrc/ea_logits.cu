@@ -1,25 +1,25 @@
 // Penalties for repeated tokens, biases and grammar masks on logits (ea_process_logits_cuda).
 //
-// Bound by HBM: a row's logits are read once and written once. A block owns a chunk of one row's vocabulary. It
-// streams the chunk through, setting what the mask forbids to -inf, and corrects the few tokens that penalties or
-// biases change afterwards. Which these are is in a table of one 32-bit word per token of the chunk in shared memory,
-// built from the row's history, path and bias list while the first logits are on their way:
-//   bits 0-19 how often the token was generated, bits 20-30 which bias entry it has first
-//   (EA_LOGITS_MAX_BIASES - entry, 0: none), bit 31 whether the prompt holds it.
-// The words are integers, so the order of the atomics cannot change them. Whoever finds a token's word zero puts the
-// token on a list, from which the corrections are then done with full warps (in place, lanes with and without a
-// token in their part of the history took turns: 80 us for 256 rows of 131072 tokens with 4096 history entries). So the
-// dense part reads no table, and the cost of the sparse part follows the lists' lengths. Rows without penalties
-// and biases build no table.
+// Bound by HBM: a row's logits are read once and written once. Two kernels:
+//   dense_kernel   streams every row through, setting what its grammar mask forbids to -inf;
+//   sparse_kernel  a block a row: collects the tokens that penalties or biases change in a hash table in shared
+//                  memory and corrects those tokens of the output. Its table is built while the dense kernel drains
+//                  (programmatic dependent launch); only the corrections wait for it.
+// One kernel with a table of counts beside each chunk of the vocabulary was measured first: 68 us against 35 us for
+// 256 rows of 131072 16-bit logits with 4096 history entries, because every chunk scans the whole history and lanes
+// with and without a token take turns.
+// A table entry's word: bits 0-19 how often the token was generated, bits 20-30 which bias entry it has first
+// (EA_LOGITS_MAX_BIASES - entry, 0: none), bit 31 whether the prompt holds it. The words are integers, so the order of
+// the atomics cannot change them.
 #include "ea_serving.cuh"
 
 namespace ea {
 namespace serving {
 namespace {
 
-constexpr int THREADS = 512;
-constexpr int UNROLL = 4;  // 16-byte pieces a thread has in flight
-constexpr int BATCH = 8;   // history entries of a thread at a time
+constexpr int DENSE_THREADS = 256, UNROLL = 4;  // 16-byte pieces a thread has in flight
+constexpr int SPARSE_THREADS = 512, BATCH = 8;  // entries a thread works on at a time
+constexpr int MAX_SLOTS = 16384, FILL = 12288;  // table entries, and how many tokens one pass puts into them
 constexpr uint32_t COUNT = 0xFFFFFu, PROMPT = 0x80000000u;
 constexpr int CODE_SHIFT = 20;
 
@@ -28,218 +28,238 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-struct Row {
-  float rep, freq, pres;
-  const int32_t* ids;
-  const float* vals;
-  bool dup;
-};
-
-// The row's rule for one token whose table word is not zero.
-__device__ __forceinline__ float adjust(float x, uint32_t w, int token, const Row& r, int num_biases) {
-  const uint32_t cnt = w & COUNT, code = (w >> CODE_SHIFT) & 0x7FFu;
-  if (cnt || (w & PROMPT)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
-  x = __fsub_rn(x, __fmul_rn(r.freq, (float)cnt));
-  if (cnt) x = __fsub_rn(x, r.pres);
-  if (code) {
-    int e = EA_LOGITS_MAX_BIASES - (int)code;
-    x = __fadd_rn(x, r.vals[e]);
-    if (r.dup)
-      for (++e; e < num_biases; ++e)
-        if (r.ids[e] == token) x = __fadd_rn(x, r.vals[e]);
-  }
-  return x;
+// The row's mask bits, nullptr where every token is allowed.
+__device__ __forceinline__ const uint32_t* mask_of(const ea_process_logits_t& a, int64_t row) {
+  if (!a.allowed_bits) return nullptr;
+  const int b = a.row_seq ? a.row_seq[row] : (int)row;
+  const int m = a.mask_rows ? a.mask_rows[row] : (int)row;
+  return b >= 0 && b < a.batch && m >= 0 && m < a.num_masks ? (const uint32_t*)a.allowed_bits + m * a.mask_stride : nullptr;
 }
 
+// Thread `tid` of `threads` streams pieces tid, tid + threads, .. (UNROLL of them) of a row from piece `first` on.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(THREADS, 2) logits_kernel(ea_process_logits_t a, int chunk, FastDiv by_chunks,
-                                                            int chunks) {
+__device__ __forceinline__ void stream_row(const ea_process_logits_t& a, int64_t row, const uint32_t* bits, int first, int tid,
+                                           int threads) {
   using P = Pack<T, VEC>;
-  extern __shared__ uint4 table4[];
-  uint32_t* table = (uint32_t*)table4;
-  uint16_t* list = (uint16_t*)(table + chunk);  // tokens with a nonzero word
-  __shared__ int dup, listed;
-  const int tid = threadIdx.x;
-  const int64_t row = div_by(blockIdx.x, by_chunks);
-  const int part = (int)(blockIdx.x - row * chunks);
   const T* src = (const T*)a.logits + row * a.logits_stride;
   T* dst = (T*)a.out + row * a.out_stride;
-  // Pieces are aligned in memory: place i of the chunk is token v0 + i, and the row's first piece may
-  // begin before its first token.
-  const int mis = (int)(((uintptr_t)src / sizeof(T)) % VEC);
-  const int v0 = part * chunk - mis;
-  if (v0 >= a.vocab) return;
-
+  // Pieces are aligned in memory, so the row's first one may begin before its first token.
+  const int v0 = (first + tid) * VEC - (int)(((uintptr_t)src / sizeof(T)) % VEC);
   P x[UNROLL];
 #pragma unroll
   for (int j = 0; j < UNROLL; ++j) {
-    const int i = (j * THREADS + tid) * VEC, v = v0 + i;
-    if (i < chunk && v >= 0 && v + VEC <= a.vocab) x[j] = *(const P*)(src + v);
+    const int v = v0 + j * threads * VEC;
+    if (v >= 0 && v + VEC <= a.vocab) x[j] = *(const P*)(src + v);
   }
+#pragma unroll
+  for (int j = 0; j < UNROLL; ++j) {
+    const int v = v0 + j * threads * VEC;
+    if (v >= a.vocab || v + VEC <= 0) continue;
+    const bool whole = v >= 0 && v + VEC <= a.vocab;
+    if (!whole) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (v + e >= 0 && v + e < a.vocab) x[j].v[e] = src[v + e];
+    }
+    if (bits) {
+      // bit e of `no`: token v + e is forbidden; the piece may lie in two words
+      const int lo = max(v, 0), hi = min(v + VEC, a.vocab) - 1;
+      const uint32_t no = ~__funnelshift_r(bits[lo >> 5], bits[hi >> 5], lo & 31) << (lo - v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if ((no >> e) & 1) x[j].v[e] = from_f<T>(-INFINITY);
+    }
+    if (whole) {
+      *(P*)(dst + v) = x[j];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (v + e >= 0 && v + e < a.vocab) dst[v + e] = x[j].v[e];
+    }
+  }
+}
 
+template <typename T, int VEC>
+__global__ void __launch_bounds__(DENSE_THREADS) dense_kernel(ea_process_logits_t a, FastDiv by_chunks, int chunks) {
+  cudaTriggerProgrammaticLaunchCompletion();
+  const int64_t row = div_by(blockIdx.x, by_chunks);
+  const int part = (int)(blockIdx.x - row * chunks);
+  stream_row<T, VEC>(a, row, mask_of(a, row), part * UNROLL * DENSE_THREADS, threadIdx.x, DENSE_THREADS);
+}
+
+// VEC 0: the dense kernel has written the rows; else this block streams its row itself.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(SPARSE_THREADS) sparse_kernel(ea_process_logits_t a, int slots, int shift) {
+  extern __shared__ uint32_t keys[];  // token + 1, 0: free; then the words
+  uint32_t* words = keys + slots;
+  __shared__ int dup;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
   const int b = a.row_seq ? a.row_seq[row] : (int)row;
   const bool real = b >= 0 && b < a.batch;
-  const int m = a.allowed_bits && real ? (a.mask_rows ? a.mask_rows[row] : (int)row) : -1;
-  const uint32_t* bits = m >= 0 && m < a.num_masks ? (const uint32_t*)a.allowed_bits + m * a.mask_stride : nullptr;
-  Row r;
-  r.rep = real && a.repetition ? a.repetition[b] : 1.0f;
-  r.freq = real && a.frequency ? a.frequency[b] : 0.0f;
-  r.pres = real && a.presence ? a.presence[b] : 0.0f;
-  const bool counts = real && (r.rep != 1.0f || r.freq != 0.0f || r.pres != 0.0f) && (a.history || a.draft_tokens);
-  const bool biased = real && a.num_biases > 0;
-  const bool tabled = counts || biased;
-  // the chunk's tokens, and the lists: history, path (drafted tokens), biases
-  const uint32_t lo = (uint32_t)max(v0, 0), span = (uint32_t)(min(a.vocab, v0 + chunk)) - lo;
-  int n_hist = 0, n_prompt = 0, n_path = 0;
-  const int32_t *hist = nullptr, *path = nullptr;
-  const uint32_t* seen = nullptr;
-  bool hist4 = false;
-  uint32_t tok[BATCH];  // places in the chunk of the thread's first history entries (>= span: elsewhere)
-  // entries first + 4 (512 j + tid) + 0 .. 3, j = 0, 1
-  const auto fetch = [&](int first) {
+  // the first history entries, asked for before their number is known
+  const int32_t* hist = a.history ? a.history + (int64_t)(real ? b : 0) * a.history_stride : nullptr;
+  uint32_t tok[BATCH];
+  const auto fetch = [&](int first, int n) {
 #pragma unroll
-    for (int j = 0; j < BATCH / 4; ++j) {
-      const int i = first + 4 * (j * THREADS + tid);
-      int4 h = make_int4(-1, -1, -1, -1);
-      if (hist4 && i + 4 <= a.max_history) {
-        h = *(const int4*)(hist + i);
-      } else {
-        if (i < a.max_history) h.x = hist[i];
-        if (i + 1 < a.max_history) h.y = hist[i + 1];
-        if (i + 2 < a.max_history) h.z = hist[i + 2];
-        if (i + 3 < a.max_history) h.w = hist[i + 3];
-      }
-      tok[4 * j] = (uint32_t)h.x - lo, tok[4 * j + 1] = (uint32_t)h.y - lo;
-      tok[4 * j + 2] = (uint32_t)h.z - lo, tok[4 * j + 3] = (uint32_t)h.w - lo;
+    for (int e = 0; e < BATCH; ++e) {
+      const int i = first + e * SPARSE_THREADS + tid;
+      tok[e] = i < n ? (uint32_t)hist[i] : 0xFFFFFFFFu;
     }
   };
-  const auto entry = [&](int first, int e) { return first + 4 * ((e >> 2) * THREADS + tid) + (e & 3); };
-  // puts a token on the list if its word was zero before
-  const auto touch = [&](uint32_t t, uint32_t before) {
-    if (before) return;
-    const uint32_t together = __activemask(), below = together & ((1u << (tid & 31)) - 1);
-    int at = 0;
-    if (!below) at = atomicAdd(&listed, __popc(together));
-    at = __shfl_sync(together, at, __ffs(together) - 1);
-    list[at + __popc(below)] = (uint16_t)t;
+  if (real && hist) fetch(0, a.max_history);
+  const uint32_t* bits = mask_of(a, row);
+  const float rep = real && a.repetition ? a.repetition[b] : 1.0f, freq = real && a.frequency ? a.frequency[b] : 0.0f,
+              pres = real && a.presence ? a.presence[b] : 0.0f;
+  const bool counts = rep != 1.0f || freq != 0.0f || pres != 0.0f;
+  // the lists: history, path (drafted tokens), biases
+  const int n_hist = counts && hist ? min(max(a.history_lens[b], 0), a.max_history) : 0;
+  const int n_prompt = n_hist && a.prompt_lens ? min(max(a.prompt_lens[b], 0), n_hist) : 0;
+  int n_path = 0;
+  const int32_t* path = nullptr;
+  if (counts && a.draft_tokens) {
+    const int64_t q0 = a.q_start[b], q1 = min((int64_t)a.q_start[b + 1], a.rows);
+    if (q0 >= 0 && q0 < q1) {
+      n_path = (int)max(min(min(q1 - q0, (int64_t)EA_LOGITS_MAX_PATH), a.tree_mask ? (int64_t)a.tree_words * 32 : row - q0 + 1), (int64_t)0);
+      path = a.draft_tokens + q0;
+    }
+  }
+  const uint32_t* seen = a.tree_mask ? (const uint32_t*)a.tree_mask + row * a.tree_words : nullptr;
+  const int n_bias = real ? a.num_biases : 0;
+  const int32_t* ids = a.bias_ids + (int64_t)b * n_bias;
+  const float* vals = a.bias_values + (int64_t)b * n_bias;
+  const int64_t all = (int64_t)n_hist + n_path + n_bias;
+  if (VEC == 0 && all == 0) {
+    cudaGridDependencySynchronize();  // nothing after this kernel may overtake the dense one
+    return;
+  }
+  // One pass where the lists fit; else as many as the vocabulary needs, pass p taking the tokens that are p modulo
+  // their number, so that no pass can overfill the table.
+  const uint32_t vocab = (uint32_t)a.vocab, passes = all <= slots / 4 * 3 ? 1u : (vocab + FILL - 1) / FILL;
+  const auto slot_of = [&](uint32_t t) -> uint32_t* {
+    for (uint32_t h = (t * 2654435761u) >> shift;; h = (h + 1) & (uint32_t)(slots - 1)) {
+      uint32_t k = keys[h];
+      if (k == 0) k = atomicCAS(keys + h, 0u, t + 1);
+      if (k == 0 || k == t + 1) return words + h;
+    }
   };
-  if (tabled) {
-    if (counts && a.history) {
-      hist = a.history + (int64_t)b * a.history_stride;
-      hist4 = ((uintptr_t)hist & 15) == 0;
-      fetch(0);
-      n_hist = min(max(a.history_lens[b], 0), a.max_history);
-      n_prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), n_hist) : 0;
-    }
-    if (counts && a.draft_tokens) {
-      const int64_t q0 = a.q_start[b], q1 = min((int64_t)a.q_start[b + 1], a.rows);
-      if (q0 >= 0 && q0 < q1) {
-        n_path = (int)min(min(q1 - q0, (int64_t)(a.tree_mask ? a.tree_words * 32 : row - q0 + 1)), (int64_t)EA_LOGITS_MAX_PATH);
-        path = a.draft_tokens + q0;
-        if (a.tree_mask) seen = (const uint32_t*)a.tree_mask + row * a.tree_words;
-      }
-    }
-    r.ids = a.bias_ids + (int64_t)b * a.num_biases;
-    r.vals = a.bias_values + (int64_t)b * a.num_biases;
-    for (int i = tid; i < (int)(span + 3) / 4; i += THREADS) table4[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) dup = listed = 0;
+  for (uint32_t pass = 0; pass < passes; ++pass) {
+    const auto mine = [&](uint32_t t) { return t < vocab && (passes == 1 || t % passes == pass); };
+    for (int i = tid; i < slots / 2; i += SPARSE_THREADS) ((uint4*)keys)[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) dup = 0;
     __syncthreads();
-    for (int first = 0; first < n_hist; first += BATCH * THREADS) {
-      if (first) fetch(first);
+    for (int first = 0; first < n_hist; first += BATCH * SPARSE_THREADS) {
+      if (first || pass) fetch(first, n_hist);
 #pragma unroll
       for (int e = 0; e < BATCH; ++e) {
-        const int i = entry(first, e);
-        if (tok[e] < span && i < n_hist) {
-          touch(tok[e], i < n_prompt ? atomicOr(table + tok[e], PROMPT) : atomicAdd(table + tok[e], 1u));
-        }
+        const int i = first + e * SPARSE_THREADS + tid;
+        if (i >= n_hist || !mine(tok[e])) continue;
+        if (i < n_prompt) atomicOr(slot_of(tok[e]), PROMPT);
+        else atomicAdd(slot_of(tok[e]), 1u);
       }
     }
-    for (int j = tid; j < n_path; j += THREADS) {
+    for (int j = tid; j < n_path; j += SPARSE_THREADS) {
       if (seen && !((seen[j >> 5] >> (j & 31)) & 1)) continue;
-      const uint32_t t = (uint32_t)path[j] - lo;
-      if (t < span) touch(t, atomicAdd(table + t, 1u));
+      const uint32_t t = (uint32_t)path[j];
+      if (mine(t)) atomicAdd(slot_of(t), 1u);
     }
     __syncthreads();
-    if (biased) {
-      for (int e = tid; e < a.num_biases; e += THREADS) {
-        const uint32_t t = (uint32_t)r.ids[e] - lo;
-        if (t < span) {
-          const uint32_t code = (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT;
-          const uint32_t old = atomicMax(table + t, (table[t] & (PROMPT | COUNT)) | code);
-          if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
-          touch(t, old);
+    for (int e = tid; e < n_bias; e += SPARSE_THREADS) {
+      const uint32_t t = (uint32_t)ids[e];
+      if (!mine(t)) continue;
+      uint32_t* w = slot_of(t);
+      const uint32_t old = atomicMax(w, (*w & (PROMPT | COUNT)) | (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT);
+      if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
+    }
+    __syncthreads();
+    // values and mask words of up to BATCH entries a thread at a time
+    for (int i0 = tid; i0 < slots; i0 += BATCH * SPARSE_THREADS) {
+      T old[BATCH];
+      uint32_t mask[BATCH];
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        const int i = i0 + e * SPARSE_THREADS;
+        tok[e] = i < slots ? keys[i] : 0;
+        mask[e] = 0xFFFFFFFFu;
+        if (tok[e]) {
+          const uint32_t t = tok[e] - 1;
+          old[e] = ((const T*)a.logits)[row * a.logits_stride + t];
+          if (bits) mask[e] = bits[t >> 5];
         }
       }
-    }
-  }
-
-  for (int i0 = 0; i0 < chunk; i0 += UNROLL * THREADS * VEC) {
-    if (i0) {
+      if (pass == 0 && i0 == tid) {  // the row is written
+        if constexpr (VEC == 0) cudaGridDependencySynchronize();
+        else {
+          const int pieces = (int)((vocab + 2 * VEC - 2) / VEC);
+          for (int first = 0; first < pieces; first += UNROLL * SPARSE_THREADS)
+            stream_row<T, VEC>(a, row, bits, first, tid, SPARSE_THREADS);
+          __syncthreads();
+        }
+      }
 #pragma unroll
-      for (int j = 0; j < UNROLL; ++j) {
-        const int i = i0 + (j * THREADS + tid) * VEC, v = v0 + i;
-        if (i < chunk && v >= 0 && v + VEC <= a.vocab) x[j] = *(const P*)(src + v);
+      for (int e = 0; e < BATCH; ++e) {
+        const uint32_t t = tok[e] - 1;
+        if (!tok[e] || !((mask[e] >> (t & 31)) & 1)) continue;
+        const uint32_t w = words[i0 + e * SPARSE_THREADS], cnt = w & COUNT, code = (w >> CODE_SHIFT) & 0x7FFu;
+        float x = to_f(old[e]);
+        if (cnt || (w & PROMPT)) x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+        x = __fsub_rn(x, __fmul_rn(freq, (float)cnt));
+        if (cnt) x = __fsub_rn(x, pres);
+        if (code) {
+          int f = EA_LOGITS_MAX_BIASES - (int)code;
+          x = __fadd_rn(x, vals[f]);
+          if (dup)
+            for (++f; f < n_bias; ++f)
+              if ((uint32_t)ids[f] == t) x = __fadd_rn(x, vals[f]);
+        }
+        ((T*)a.out)[row * a.out_stride + t] = from_f<T>(x);
       }
     }
-#pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      const int i = i0 + (j * THREADS + tid) * VEC, v = v0 + i;
-      if (i >= chunk || v >= a.vocab || v + VEC <= 0) continue;
-      const bool whole = v >= 0 && v + VEC <= a.vocab;
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (v + e >= 0 && v + e < a.vocab) x[j].v[e] = src[v + e];
-      }
-      if (bits) {
-        // bit e of `no`: token v + e is forbidden; the piece may lie in two words
-        const int first = max(v, 0), last = min(v + VEC, a.vocab) - 1;
-        uint32_t no = ~__funnelshift_r(bits[first >> 5], bits[last >> 5], first & 31) << (first - v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if ((no >> e) & 1) x[j].v[e] = from_f<T>(-INFINITY);
-      }
-      if (whole) {
-        *(P*)(dst + v) = x[j];
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (v + e >= 0 && v + e < a.vocab) dst[v + e] = x[j].v[e];
-      }
-    }
-  }
-  if (!tabled) return;
-
-  __syncthreads();  // the chunk is written and the table complete
-  r.dup = dup != 0;
-  for (int i = tid; i < listed; i += THREADS) {
-    const uint32_t t = list[i];
-    const int v = (int)(lo + t);
-    if (bits && !((bits[v >> 5] >> (v & 31)) & 1)) continue;
-    dst[v] = from_f<T>(adjust(to_f(src[v]), table[t], v, r, a.num_biases));
+    __syncthreads();
   }
 }
 
 template <typename T, int VEC>
 int launch(const ea_process_logits_t& a, cudaStream_t st) {
-  // The largest chunk whose blocks still fill the GPU twice: fewer chunks read the history less often.
-  int chunk = 16384;
-  while (chunk > 2048 && a.rows * ((a.vocab + chunk - 1) / chunk) < 2 * sm_count()) chunk >>= 1;
-  const int chunks = (int)(((int64_t)a.vocab + VEC - 1 + chunk - 1) / chunk);
-  chunk = (int)((((int64_t)a.vocab + VEC - 1 + chunks - 1) / chunks + 15) & ~15ll);  // equal chunks
-  const int64_t blocks = a.rows * chunks;
-  if (blocks > 0x7FFFFFFF) return fail(-1, "process_logits: too many rows");
-  const size_t smem = (size_t)chunk * 6;
-  static bool ready[64];  // per device
+  const bool counts = (a.repetition || a.frequency || a.presence) && (a.history || a.draft_tokens);
+  const bool sparse = counts || a.num_biases, dense = a.allowed_bits || a.out != a.logits;
+  // Few short rows: a block that streams its row before it corrects it saves the second launch (6 us against 9 us for one
+  // row of 32000 tokens).
+  const bool together = sparse && dense && a.rows <= sm_count() && a.vocab <= 3 * UNROLL * SPARSE_THREADS * VEC;
+  if (dense && !together) {
+    const int per_block = UNROLL * DENSE_THREADS * VEC;
+    const int chunks = (int)(((int64_t)a.vocab + VEC - 1 + per_block - 1) / per_block);
+    const int64_t blocks = a.rows * chunks;
+    if (blocks >= (1ll << 31)) return fail(-1, "process_logits: too many rows");
+    dense_kernel<T, VEC><<<(unsigned)blocks, DENSE_THREADS, 0, st>>>(a, fast_div((uint32_t)chunks), chunks);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_rc(e);
+  }
+  if (!sparse) return 0;
+  // table: four thirds of the longest lists the sizes allow, at most MAX_SLOTS (then several passes)
+  const int64_t longest = (int64_t)a.max_history + a.num_biases + (a.draft_tokens ? (a.tree_mask ? a.tree_words * 32 : 1024) : 0);
+  int log2 = 10;
+  while ((1 << log2) < MAX_SLOTS && (1 << log2) / 4 * 3 < longest) ++log2;
+  const int slots = 1 << log2;
+  const auto kernel = together ? sparse_kernel<T, VEC> : sparse_kernel<T, 0>;
+  static bool ready[2][64];  // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
-    e = cudaFuncSetAttribute(logits_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 6 * 16400);
-    if (e == cudaSuccess && dev < 64) ready[dev] = true;
+  if (e == cudaSuccess && (dev >= 64 || !ready[together][dev])) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SLOTS * 8);
+    if (e == cudaSuccess && dev < 64) ready[together][dev] = true;
   }
   if (e != cudaSuccess) return cuda_rc(e);
-  logits_kernel<T, VEC><<<(unsigned)blocks, THREADS, smem, st>>>(a, chunk, fast_div((uint32_t)chunks), chunks);
-  return cuda_rc(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.rows), cfg.blockDim = dim3(SPARSE_THREADS), cfg.dynamicSmemBytes = (size_t)slots * 8;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr, cfg.numAttrs = dense && !together ? 1 : 0;  // after the dense kernel only
+  e = cudaLaunchKernelEx(&cfg, kernel, a, slots, 32 - log2);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return cuda_rc(e);
 }
 
 template <typename T>

@@ -59,7 +59,7 @@ __device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
 }
 
 template <typename T, int VEC, int ITEMS, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 3 : 1) rope_kernel(ea_rope_t a, Plan p) {
+__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : ITEMS == 4 ? 3 : 5) rope_kernel(ea_rope_t a, Plan p) {
   using P = Pack<T, VEC>;
   extern __shared__ float2 cs[];  // (tokens, rot / 2)
   const uint32_t group = div_by(blockIdx.x, p.by_head_blocks);

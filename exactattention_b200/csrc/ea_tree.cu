@@ -145,6 +145,7 @@ __device__ __forceinline__ bool sees(const Args& a, const Item& it, int i, int k
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
   using S = Smem<DP>;
+  cudaTriggerProgrammaticLaunchCompletion();
   extern __shared__ uint8_t raw[];
   uint8_t* pool = (uint8_t*)(((uintptr_t)raw + 255) & ~(uintptr_t)255);
   uint32_t* sums = (uint32_t*)(raw + S::POOL);
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
         if (c < a.t.d) ((T*)a.t.out)[head * a.t.d + c] = from_f<T>(ll == 0.0f ? 0.0f : x / ll);
         if (c == 0 && a.t.lse) a.t.lse[head] = ll == 0.0f ? -INFINITY : mm + log2f(ll);
       } else {
-        slot[r * DP + c] = x;
+        slot[((c >> 2) * ROWS + r) * 4 + (c & 3)] = x;
         if (c == 0) slot[ROWS * DP + r] = mm, slot[ROWS * (DP + 1) + r] = ll;
       }
     }
@@ -415,7 +416,6 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
 template <typename T, int DP>
 int launch(Args& a, cudaStream_t st) {
   const size_t smem = Smem<DP>::POOL + 4 * (size_t)(a.t.batch + 1);
-  const size_t csmem = 4 * (size_t)(a.t.batch + 1);
   static bool ready[64];  // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -428,8 +428,7 @@ int launch(Args& a, cudaStream_t st) {
   few_rows_kernel<T, DP><<<a.workers, THREADS, smem, st>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_rc(e);
-  if (a.workers > 1) combine_kernel<T, ROWS, KT, 256><<<a.workers, 256, csmem, st>>>(a);
-  return cuda_rc(cudaGetLastError());
+  return launch_combine<T, ROWS, KT>(a, st);
 }
 
 // Most units a call can have, from the sizes the host knows.
@@ -455,15 +454,17 @@ int check(const ea_tree_attention_t* t) {
   return 0;
 }
 
-// Which kernel: query rows per sequence and kv head at most 16 (few_rows_kernel), 128, or more. max_new is a hint,
-// so any choice is right for any lengths.
+// Which kernel, by the query rows per sequence and kv head: at most 16 (few_rows_kernel), below 512 the tensor-core
+// kernel with 128-row items, else with 256-row items, which take half the traffic from L2 but keep one of two slots
+// idle where an item has 128 rows or fewer (2048 rows: 345 us against 370 us; 7 to 231 rows: 73 us against 68 us).
+// max_new is a hint, so any choice is right for any lengths.
 struct Choice {
   int rows, kt, per_sm;
 };
 Choice choose(const ea_tree_attention_t& t) {
   const int64_t rows = (int64_t)(t.max_new > 0 ? t.max_new : 1) * (t.q_heads / t.kv_heads);
   if (rows <= ROWS || t.batch > MANY_MAX_SEQS) return {ROWS, KT, 2};
-  return {rows <= 128 ? 128 : 256, 128, 1};
+  return {rows < 512 ? 128 : 256, 128, 1};
 }
 int workers_for(const ea_tree_attention_t& t, const Choice& c) {
   const int64_t most = most_units(t, c.rows, c.kt), fill = (int64_t)c.per_sm * sm_count();

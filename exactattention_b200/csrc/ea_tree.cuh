@@ -103,7 +103,8 @@ struct Schedule {
 };
 
 // A share's partials: slot 2 w is the item it began inside of (its first), slot 2 w + 1 the one it leaves
-// unfinished. Layout of a slot: ROWS x dp floats, ROWS maxima, ROWS sums.
+// unfinished. Layout of a slot: dp / 4 x ROWS x 4 floats (a row per thread stores and loads whole lines), ROWS maxima,
+// ROWS sums.
 __device__ __forceinline__ float* slot_of(const Args& a, int slot, int rows) {
   return (float*)a.t.workspace + (int64_t)slot * rows * (a.dp + 2);
 }
@@ -112,45 +113,127 @@ __device__ __forceinline__ float* slot_of(const Args& a, int slot, int rows) {
 constexpr int MANY_MAX_SEQS = 6000;  // what its shared memory has room for
 int launch_many(const Args& a, bool pair, cudaStream_t st);
 
-// Adds up the partials of the item that share blockIdx.x left unfinished, 16 rows a block (blockIdx.y).
-template <typename T, int ROWS, int KT, int THREADS>
-__global__ void __launch_bounds__(THREADS) combine_kernel(Args a) {
+// Adds up the partials of the item that share blockIdx.x left unfinished, 16 rows a block (blockIdx.y). It starts
+// while the attention kernel still runs (programmatic dependent launch) and finds its item meanwhile.
+// Thread (share group, row, four channels): the groups take every G-th share, with all of a row's weights
+// 2^(m - max) computed once; the groups' sums are joined in a fixed order.
+constexpr int COMBINE_THREADS = 256, COMBINE_SHARES = 64;  // shares whose weights are held at a time
+
+template <typename T, int ROWS, int KT>
+__global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(Args a) {
   extern __shared__ uint32_t sums[];
   __shared__ uint64_t scratch[32];
+  __shared__ float weight[COMBINE_SHARES][16], top[16], total[16];
+  __shared__ float4 joined[COMBINE_THREADS];
   Schedule<ROWS, KT> sch;
   sch.build(a, sums, scratch);
-  const int w = blockIdx.x;
+  const int w = blockIdx.x, tid = threadIdx.x, r0 = blockIdx.y * 16;
   const uint32_t lo = sch.share(w), hi = sch.share(w + 1);
-  if (lo >= hi) return;
-  const Item it = sch.item(a, hi - 1, hi);
-  const uint32_t begin = hi - 1 - it.kt0;  // the item's first unit
-  const uint32_t end = begin + it.tiles;
-  if (begin < lo || end <= hi) return;  // begun earlier, or finished here
-  int last = w;
-  while (sch.share(last + 1) < end) ++last;
-  const int r0 = blockIdx.y * 16, rows = min(16, min(ROWS, it.new_tokens * a.group - it.m * ROWS) - r0);
-  const int stride = ROWS * (a.dp + 2);
-  const float* first = slot_of(a, 2 * w + 1, ROWS);
-  const float* rest = slot_of(a, 2 * w, ROWS);  // share w' > w: rest + (w' - w) * 2 * stride
-  const int cols = a.dp;
-  for (int e = threadIdx.x; e < rows * cols; e += THREADS) {
-    const int r = r0 + e / cols, c = e % cols;
-    float m = first[ROWS * a.dp + r];
-    for (int i = 1; i <= last - w; ++i) m = fmaxf(m, rest[(int64_t)i * 2 * stride + ROWS * a.dp + r]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float s = exp2f(first[ROWS * a.dp + r] - base);
-    float l = first[ROWS * (a.dp + 1) + r] * s, o = first[r * a.dp + c] * s;
-    for (int i = 1; i <= last - w; ++i) {
-      const float* p = rest + (int64_t)i * 2 * stride;
-      s = exp2f(p[ROWS * a.dp + r] - base);
-      l = fmaf(p[ROWS * (a.dp + 1) + r], s, l);
-      o = fmaf(p[r * a.dp + c], s, o);
+  Item it;
+  int rows = 0, n = 2;  // rows of this block, shares of the item
+  if (lo < hi) {
+    it = sch.item(a, hi - 1, hi);
+    const uint32_t begin = hi - 1 - it.kt0, end = begin + it.tiles;  // the item's units
+    if (begin >= lo && end > hi) {                                   // begun here and not finished here
+      rows = min(16, min(ROWS, it.new_tokens * a.group - it.m * ROWS) - r0);
+      while (sch.share(w + n) < end) ++n;
     }
-    const int R = it.m * ROWS + r, i = (int)div_by((uint32_t)R, a.by_group), j = R - i * a.group;
-    const int64_t head = (int64_t)(it.q0 + i) * a.t.q_heads + it.h * a.group + j;
-    if (c < a.t.d) ((T*)a.t.out)[head * a.t.d + c] = from_f<T>(l == 0.0f ? 0.0f : o / l);
-    if (c == 0 && a.t.lse) a.t.lse[head] = l == 0.0f ? -INFINITY : m + log2f(l);
   }
+  cudaGridDependencySynchronize();
+  if (rows <= 0) return;
+  // partial i of the item: slot 2 w + 1, then slots 2 (w + i)
+  const auto part = [&](int i) { return slot_of(a, i ? 2 * (w + i) : 2 * w + 1, ROWS); };
+
+  // maxima of the rows: 16 lanes a row
+  {
+    const int r = tid >> 4;
+    float m = -INFINITY;
+    if (r < rows)
+      for (int i = tid & 15; i < n; i += 16) m = fmaxf(m, part(i)[ROWS * a.dp + r0 + r]);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((tid & 15) == 0) top[r] = m, total[r] = 0.0f;
+  }
+  const int vecs = a.dp / 4, cells = rows * vecs;  // at most 512: two cells a thread where there are many rows
+  int groups = COMBINE_THREADS / cells;            // groups of threads that take every groups-th share
+  if (groups < 1) groups = 1;
+  const int grp = min(tid / cells, groups), cell0 = cells > COMBINE_THREADS ? tid : tid - tid / cells * cells;
+  float4 acc[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+  for (int i0 = 0; i0 < n; i0 += COMBINE_SHARES) {
+    const int m = min(COMBINE_SHARES, n - i0);
+    __syncthreads();
+    {
+      const int r = tid >> 4;
+      float l = 0.0f;
+      if (r < rows) {
+        const float base = top[r] == -INFINITY ? 0.0f : top[r];
+        for (int i = tid & 15; i < m; i += 16) {
+          const float* p = part(i0 + i) + ROWS * a.dp + r0 + r;
+          const float f = exp2f(p[0] - base);
+          weight[i][r] = f;
+          l = fmaf(p[ROWS], f, l);
+        }
+      }
+#pragma unroll
+      for (int o = 8; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      if ((tid & 15) == 0) total[r] += l;
+    }
+    __syncthreads();
+    if (grp < groups)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int cell = cell0 + c * COMBINE_THREADS;
+        if (cell >= cells) break;
+        const int v = cell / rows, r = cell - v * rows, at = (v * ROWS + r0 + r) * 4;
+#pragma unroll 4
+        for (int i = grp; i < m; i += groups) {
+          const float4 x = *(const float4*)(part(i0 + i) + at);
+          const float f = weight[i][r];
+          acc[c].x = fmaf(x.x, f, acc[c].x), acc[c].y = fmaf(x.y, f, acc[c].y);
+          acc[c].z = fmaf(x.z, f, acc[c].z), acc[c].w = fmaf(x.w, f, acc[c].w);
+        }
+      }
+  }
+  if (groups > 1) {
+    joined[tid] = acc[0];
+    __syncthreads();
+    if (tid < cells)
+      for (int g = 1; g < groups; ++g) {
+        const float4 x = joined[g * cells + tid];
+        acc[0].x += x.x, acc[0].y += x.y, acc[0].z += x.z, acc[0].w += x.w;
+      }
+  }
+  if (grp > 0) return;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int cell = cell0 + c * COMBINE_THREADS;
+    if (cell >= cells) break;
+    const int v = cell / rows, r = cell - v * rows, ch = v * 4;
+    const int R = it.m * ROWS + r0 + r, i = (int)div_by((uint32_t)R, a.by_group), j = R - i * a.group;
+    const int64_t head = (int64_t)(it.q0 + i) * a.t.q_heads + it.h * a.group + j;
+    const float l = total[r], inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (ch < a.t.d) {  // d is a multiple of 8
+      T y[4] = {from_f<T>(acc[c].x * inv), from_f<T>(acc[c].y * inv), from_f<T>(acc[c].z * inv), from_f<T>(acc[c].w * inv)};
+      *(uint2*)((T*)a.t.out + head * a.t.d + ch) = *(const uint2*)y;
+    }
+    if (ch == 0 && a.t.lse) a.t.lse[head] = l == 0.0f ? -INFINITY : top[r] + log2f(l);
+  }
+}
+
+// Launches the combine kernel right after an attention kernel on the stream.
+template <typename T, int ROWS, int KT>
+int launch_combine(const Args& a, cudaStream_t st) {
+  if (a.workers <= 1) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.workers, ROWS / 16), cfg.blockDim = dim3(COMBINE_THREADS);
+  cfg.dynamicSmemBytes = 4 * (size_t)(a.t.batch + 1), cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, combine_kernel<T, ROWS, KT>, a);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return cuda_rc(e);
 }
 
 }  // namespace tree

@@ -19,6 +19,8 @@
 // Weights are rounded to the cache's type for the product (relative error 2^-9 for bf16, 2^-12 for fp16, of
 // random sign, about the rounding of the output itself); their sum takes them unrounded.
 #pragma once
+#include <cuda.h>
+
 #include "ea_tcgen05.cuh"
 #include "ea_tree.cuh"
 
@@ -29,8 +31,10 @@ namespace many {
 
 using namespace ea::tc;
 
-constexpr int KT = 128, TILE = 128, THREADS = 512;
-constexpr int SLOT_THREADS = 128, LOADERS = 128;
+constexpr int KT = 128, TILE = 128, THREADS = 384;  // warps 0-7 softmax slots, 8 products, 9-11 copies
+constexpr int SLOT_THREADS = 128, LOADERS = 64;
+// registers a thread: at launch, and after the groups have traded (2 x 128 x 216 + 128 x 72 = 384 x 168)
+constexpr int LAUNCH_REGS = 168, SLOT_REGS = 216, OTHER_REGS = 72;
 constexpr uint32_t COL_S = 0, COL_O = 256;  // slot s: + 128 s
 constexpr int PAGE_RING = 16;
 
@@ -44,11 +48,11 @@ struct Cfg {
 };
 
 struct Shared {
-  uint64_t full[8], empty[8], s_full[2], p_ready[2], q_full, done;
+  uint64_t full[8], empty[8], s_full[2], p_ready[2], q_full, q_free, seen, done;
   uint64_t scratch[32];
   uint32_t tmem;
   uint32_t page_ok[PAGE_RING][4];
-  int dirty[2];
+  int dirty[2][2];  // item parity, slot
   float m[2][TILE], l[2][TILE];
 };
 
@@ -58,29 +62,61 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
          ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
 }
 
-// shared-memory descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart; `lbo`: distance between the 64-element
-// blocks of an MN-major operand
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024u >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
+// Low word of a shared-memory descriptor: start address, and for an MN-major operand the distance `lbo` between its
+// 64-element blocks. The high word is the same for all: 8-row groups 1024 bytes apart, version 1, 128-byte swizzle.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
+constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+// One product step, issued by the lane whose `leader` is set; the warp stays together, so that the operands stay in
+// uniform registers (a branch to one lane made an issue cost 100-300 cycles instead of the product's 64).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(acc ? 1u : 0u)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 da, {%1, %6};\n\tmov.b64 db, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(acc), "r"(leader), "r"(DESC_HI)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc ? 1u : 0u)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 db, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(acc), "r"(leader), "r"(DESC_HI)
       : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+// Bounded wait that reads the timer only when the phase is late (a read costs some 300 cycles).
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_u32(bar);
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(a), "r"(parity), "r"(10000u)
+        : "memory");
+    if (done) return true;
+  }
+  return mbar_wait(bar, parity);
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// 4D tiled tensor load; x times the element size is a multiple of 16 bytes, what lies outside the tensor reads as zeros
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ bool try_now(uint64_t* bar, uint32_t parity) {
   uint32_t done;
@@ -103,6 +139,19 @@ __device__ __forceinline__ void ld32(uint32_t addr, uint32_t* v) {
       : "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : EA_R8(v, 0), EA_R8(v, 8)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      EA_I8(v, 0), EA_I8(v, 8)
+      : "memory");
+}
 __device__ __forceinline__ void st32(uint32_t addr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -110,10 +159,43 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t* v) {
       EA_I8(v, 0), EA_I8(v, 8), EA_I8(v, 16), EA_I8(v, 24)
       : "memory");
 }
+#define EA_W8(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7])
+// waits for this thread's loads; the 16 registers are named so that nothing reads them earlier
+__device__ __forceinline__ void wait_ld16(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : EA_W8(v, 0), EA_W8(v, 8)::"memory");
+}
+// -inf in the places whose bit is clear
+__device__ __forceinline__ void hide16(uint32_t* v, uint32_t seen) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (!((seen >> e) & 1)) v[e] = 0xFF800000u;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two binary32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
@@ -196,7 +278,9 @@ __device__ __noinline__ void add_not_finite(const Args& a, const Item& it, int i
 }
 
 template <typename T, int DP, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
+__global__ void __launch_bounds__(THREADS, 1)
+    many_rows_kernel(Args a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, int box) {
+  cudaTriggerProgrammaticLaunchCompletion();
   using C = Cfg<DP, PAIR>;
   constexpr int ROWS = C::ROWS, NBUF = C::NBUF, BUF = C::BUF;
   extern __shared__ uint8_t raw[];
@@ -210,11 +294,11 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
   Schedule<ROWS, KT> sch;
   sch.build(a, sums, sh.scratch);
   if (tid == 0) {
-    for (int i = 0; i < NBUF; ++i) mbar_init(&sh.full[i], LOADERS), mbar_init(&sh.empty[i], 1);
+    for (int i = 0; i < NBUF; ++i) mbar_init(&sh.full[i], box ? 1 : LOADERS), mbar_init(&sh.empty[i], 1);
     for (int s = 0; s < 2; ++s) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], SLOT_THREADS);
-    mbar_init(&sh.q_full, 2 * SLOT_THREADS);
+    mbar_init(&sh.q_full, 32), mbar_init(&sh.q_free, 1), mbar_init(&sh.seen, 2 * SLOT_THREADS);
     mbar_init(&sh.done, 1);
-    sh.dirty[0] = sh.dirty[1] = 0;
+    sh.dirty[0][0] = sh.dirty[0][1] = sh.dirty[1][0] = sh.dirty[1][1] = 0;
   }
   if (warp == 8) tmem_alloc(&sh.tmem, 512);
   fence_before_sync();
@@ -225,10 +309,101 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
   const uint32_t end = sch.share(blockIdx.x + 1);
   bool alive = true;  // false once a bounded wait gave up: no more waits, products or copies; the rows become NaN
 
-  if (warp >= 12) {
-    // ---- loaders: every thread copies 16-byte pieces of every tile, in the order the products use them
-    set_regs<64, false>();
-    const int w4 = warp - 12, key_lane = w4 * 32 + lane;
+  // order in which the tiles are loaded and used: PAIR K0, then V(t), K(t + 1); else K0, K1, then V(t), K(t + 2)
+  constexpr int AHEAD = PAIR ? 1 : 2;
+  if (warp >= 8) set_regs<OTHER_REGS, false>();
+  if (warp == (box ? 10 : 9)) {
+    // ---- query rows of the next item, as soon as the last scores of this one are computed
+    uint32_t items = 0;
+    while (pos < end && alive) {
+      const Item it = sch.item(a, pos, end);
+      pos += it.kt1 - it.kt0;
+      if (items) alive = __all_sync(0xffffffffu, wait_phase(&sh.q_free, (items - 1) & 1));
+      if (!alive) break;
+      ++items;
+      constexpr int PIECES = DP / 8;
+      const int rows = min(ROWS, it.new_tokens * a.group - it.m * ROWS);
+#pragma unroll 4
+      for (int e = lane; e < rows * PIECES; e += 32) {
+        const int r = e / PIECES, p = e % PIECES, R = it.m * ROWS + r, tok = (int)div_by((uint32_t)R, a.by_group);
+        const T* q = (const T*)a.t.q + (int64_t)(it.q0 + tok) * a.t.q_stride +
+                     (int64_t)(it.h * a.group + R - tok * a.group) * a.t.q_head_stride + p * 8;
+        const bool in = p * 8 < a.t.d;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(qbuf) + tile_off(r, p, ROWS)),
+                     "l"(in ? (const void*)q : a.t.q), "r"(in ? 16 : 0)
+                     : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (a.t.alpha <= 0)  // the slots work with |alpha|, and with 1 for 0
+        for (int e = lane; e < rows * PIECES; e += 32) {
+          uint32_t* w = (uint32_t*)(qbuf + tile_off(e / PIECES, e % PIECES, ROWS));
+          for (int i = 0; i < 4; ++i) w[i] = a.t.alpha < 0 ? w[i] ^ 0x80008000u : 0u;
+        }
+      fence_async_smem();
+      arrive(&sh.q_full);
+    }
+  } else if (warp >= 9 && box) {
+    // ---- loader warp, tensor copies: a lane issues one box (64 channels x `box` rows of one page) of every tile
+    if (warp == 9) {
+      constexpr int CB = DP / 64;
+      const int sub = lane / CB, cb = lane % CB;
+      const bool active = sub * box < KT;
+      uint32_t cnt = 0, tile0 = 0;  // tiles loaded; key tiles of earlier items
+      while (pos < end && alive) {
+        const Item it = sch.item(a, pos, end);
+        pos += it.kt1 - it.kt0;
+        const int n = it.kt1 - it.kt0;
+        const auto page_of = [&](int t) {
+          const int key = (it.kt0 + t) * KT + sub * box;
+          if (!active || t >= n || key >= it.len) return -1;
+          const int p = a.t.page_table[it.b * a.t.table_stride + div_by((uint32_t)key, a.by_page)];
+          return p >= 0 && p < a.t.num_pages ? p : -1;
+        };
+        const auto load = [&](int t, int page, bool value) {
+          const uint32_t b = cnt % NBUF;
+          if (cnt >= NBUF) alive = __all_sync(0xffffffffu, wait_phase(&sh.empty[b], (cnt / NBUF - 1) & 1));
+          if (!alive) return;
+          if (!value) {  // which of the tile's keys have a page
+            const uint32_t bits = page < 0 ? 0u : box >= 32 ? 0xFFFFFFFFu : ((1u << box) - 1) << (sub * box & 31);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const bool here = active && sub * box < (w + 1) * 32 && (sub + 1) * box > w * 32;
+              const uint32_t all = __reduce_or_sync(0xffffffffu, here ? bits : 0u);
+              if (lane == 0) sh.page_ok[(tile0 + t) % PAGE_RING][w] = all;
+            }
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&sh.full[b], BUF);
+          __syncwarp();
+          if (active) {
+            const int key = (it.kt0 + t) * KT + sub * box;
+            const int row = page < 0 ? 0 : key - (int)div_by((uint32_t)key, a.by_page) * a.t.page_size;
+            tma_load_4d(ring + b * BUF + cb * KT * 128 + sub * box * 128, value ? &tv : &tk, cb * 64, row, it.h,
+                        page < 0 ? (int)a.t.num_pages : page, &sh.full[b]);
+          }
+          ++cnt;
+        };
+        int page[AHEAD + 1], next = page_of(AHEAD);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) page[i] = page_of(i);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          if (i < n && alive) load(i, page[i], false);
+        for (int t = 0; t < n && alive; ++t) {
+          page[AHEAD] = next;
+          next = page_of(t + AHEAD + 1);
+          load(t, page[0], true);
+          if (t + AHEAD < n && alive) load(t + AHEAD, page[AHEAD], false);
+#pragma unroll
+          for (int i = 0; i < AHEAD; ++i) page[i] = page[i + 1];
+        }
+        tile0 += n;
+      }
+      // copies under way land before the block gives its shared memory back
+      for (uint32_t c = cnt > NBUF ? cnt - NBUF : 0; c < cnt; ++c) mbar_wait(&sh.full[c % NBUF], (c / NBUF) & 1);
+    }
+  } else if (warp >= 10) {
+    // ---- loaders, any page size: every thread copies 16-byte pieces of every tile; a lane looks up the pages of two keys
+    const int w2 = warp - 10;
     uint32_t cnt = 0, pending = 0, signalled = 0, tile0 = 0;  // tile0: tiles of earlier items
     const auto retire = [&]() {  // waits for the oldest tile in flight and hands it over
       switch (pending) {
@@ -249,177 +424,140 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
       const Item it = sch.item(a, pos, end);
       pos += it.kt1 - it.kt0;
       const int n = it.kt1 - it.kt0;
-      const auto page_of = [&](int t) {
-        const int key = (it.kt0 + t) * KT + key_lane;
+      const auto page_of = [&](int t, int half) {
+        const int key = (it.kt0 + t) * KT + w2 * 64 + half * 32 + lane;
         if (t >= n || key >= it.len) return -1;
         const int p = a.t.page_table[it.b * a.t.table_stride + div_by((uint32_t)key, a.by_page)];
         return p >= 0 && p < a.t.num_pages ? p : -1;
       };
-      const auto load = [&](int t, int page, bool value) {
+      const auto load = [&](int t, bool value) {
         const uint32_t b = cnt % NBUF;
         if (cnt >= NBUF) {
           const uint32_t parity = (cnt / NBUF - 1) & 1;
           while (pending && !__all_sync(0xffffffffu, try_now(&sh.empty[b], parity))) retire();
-          alive = __all_sync(0xffffffffu, mbar_wait(&sh.empty[b], parity));
+          alive = __all_sync(0xffffffffu, wait_phase(&sh.empty[b], parity));
           if (!alive) return;
         }
         if (pending == 7) retire();
-        if (!value) {
-          const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
-          if (lane == 0) sh.page_ok[(tile0 + t) % PAGE_RING][w4] = ok;
-        }
         const uint32_t dst = smem_u32(ring + b * BUF);
         const T* src = (const T*)(value ? a.t.v_cache : a.t.k_cache) + it.h * (value ? a.t.v_head_stride : a.t.k_head_stride);
         const int64_t ps = value ? a.t.v_page_stride : a.t.k_page_stride, rs = value ? a.t.v_row_stride : a.t.k_row_stride;
-        const int key0 = (it.kt0 + t) * KT + w4 * 32;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          const int row0 = w2 * 64 + half * 32, key0 = (it.kt0 + t) * KT + row0;
+          const int page = page_of(t, half);
+          if (!value) {
+            const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane == 0) sh.page_ok[(tile0 + t) % PAGE_RING][row0 / 32] = ok;
+          }
+#pragma unroll 2
+          for (int q = 0; q < 8; ++q) {
+            const int r = q * 4 + lane / 8;
+            const int pg = __shfl_sync(0xffffffffu, page, r);
+            const int key = key0 + r;
+            const int64_t off = pg >= 0 ? key - (int64_t)div_by((uint32_t)key, a.by_page) * a.t.page_size : 0;
+            const T* row = src + (pg >= 0 ? pg : 0) * ps + off * rs;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int r = q * 4 + lane / 8;
-          const int pg = __shfl_sync(0xffffffffu, page, r);
-          const int key = key0 + r;
-          const int64_t off = pg >= 0 ? key - (int64_t)div_by((uint32_t)key, a.by_page) * a.t.page_size : 0;
-          const T* row = src + (pg >= 0 ? pg : 0) * ps + off * rs;
-#pragma unroll
-          for (int c = 0; c < DP / 64; ++c) {
-            const int piece = c * 8 + (lane & 7);
-            const bool in = pg >= 0 && piece * 8 < a.t.d;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + tile_off(w4 * 32 + r, piece, KT)),
-                         "l"(in ? (const void*)(row + piece * 8) : (value ? a.t.v_cache : a.t.k_cache)), "r"(in ? 16 : 0)
-                         : "memory");
+            for (int c = 0; c < DP / 64; ++c) {
+              const int piece = c * 8 + (lane & 7);
+              const bool in = pg >= 0 && piece * 8 < a.t.d;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + tile_off(row0 + r, piece, KT)),
+                           "l"(in ? (const void*)(row + piece * 8) : (value ? a.t.v_cache : a.t.k_cache)), "r"(in ? 16 : 0)
+                           : "memory");
+            }
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         ++cnt, ++pending;
       };
-      // order of use: PAIR K0, then V(t), K(t + 1); else K0, K1, then V(t), K(t + 2)
-      constexpr int AHEAD = PAIR ? 1 : 2;
-      int page[AHEAD + 1], next = page_of(AHEAD);
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) page[i] = page_of(i);
-#pragma unroll
       for (int i = 0; i < AHEAD; ++i)
-        if (i < n && alive) load(i, page[i], false);
+        if (i < n && alive) load(i, false);
       for (int t = 0; t < n && alive; ++t) {
-        page[AHEAD] = next;
-        next = page_of(t + AHEAD + 1);
-        load(t, page[0], true);
-        if (t + AHEAD < n && alive) load(t + AHEAD, page[AHEAD], false);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) page[i] = page[i + 1];
+        load(t, true);
+        if (t + AHEAD < n && alive) load(t + AHEAD, false);
       }
       tile0 += n;
     }
     while (pending) retire();
   } else if (warp >= 8) {
-    // ---- the MMA thread
-    set_regs<64, false>();
-    if (warp == 8 && lane == 0) {
+    // ---- products, one lane issues them. One issuer for both slots keeps the slots half a cycle apart; with an issuer each
+    // they ran in step and waited for the same pipes at the same time (6000 cycles for a pair of tiles against 4600).
+    if (warp == 8) {
       constexpr uint32_t QK = idesc<T>(KT, false), PV = idesc<T>(DP, true);
-      uint32_t cnt = 0, items = 0, np[2] = {0, 0};
-      const uint32_t qa = smem_u32(qbuf), ra = smem_u32(ring);
+      const uint32_t leader = lane == 0;
+      uint32_t cnt = 0, items = 0, phases = 0;  // tiles taken from the ring; items; bit s: parity of slot s's weights
+      const uint32_t qd = desc_lo(smem_u32(qbuf), 16), ring_at = smem_u32(ring);
       const auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (alive && !mbar_wait(bar, parity)) alive = false;
+        if (alive) alive = __all_sync(0xffffffffu, wait_phase(bar, parity));
       };
       while (pos < end && alive) {
         const Item it = sch.item(a, pos, end);
         pos += it.kt1 - it.kt0;
         const int n = it.kt1 - it.kt0;
-        const bool two = !PAIR || it.new_tokens * a.group - it.m * ROWS > TILE;
+        const int slots = !PAIR || it.new_tokens * a.group - it.m * ROWS > TILE ? 2 : 1;  // PAIR: slots with rows
+        if (items) wait(&sh.seen, (items - 1) & 1);  // the slots have seen the end of the last item
         wait(&sh.q_full, items & 1);
         ++items;
-        const auto buf_full = [&](uint32_t c) { wait(&sh.full[c % NBUF], (c / NBUF) & 1); };
-        const auto qk = [&](int slot, uint32_t c) {
-          if (!alive) return;
-          const uint32_t qs = qa + (PAIR ? slot * TILE * 128 : 0), kb = ra + (c % NBUF) * BUF;
+        // A step: the weights of tile t times its values, then the scores of tile t + AHEAD into the same slot, then
+        // the word to the slot. PAIR: both slots take every tile; else the slot is the tile's parity.
+        const int steps = (n + AHEAD) * (PAIR ? 2 : 1);
+#pragma unroll 1
+        for (int i = 0; i < steps && alive; ++i) {
+          const int t = (PAIR ? i >> 1 : i) - AHEAD, slot = i & 1;
+          const bool idle = slot >= slots, first = !PAIR || slot == 0, last = !PAIR || slot == 1;
+          const uint32_t s_cols = tmem + COL_S + slot * 128;
+          const bool more = t + AHEAD < n;
+          const uint32_t cv = cnt, ck = PAIR && t >= 0 ? cnt + 1 : cnt;  // ring positions of V(t) and K(t + AHEAD)
+          if (t >= 0) {
+            if (first) wait(&sh.full[cv % NBUF], (cv / NBUF) & 1);
+            if (!idle) {
+              wait(&sh.p_ready[slot], phases >> slot & 1);
+              phases ^= 1u << slot;
+              fence_after_sync();
+            }
+            if (!alive) break;
+            if (!idle) {
+              const uint32_t v = desc_lo(ring_at + (cv % NBUF) * BUF, KT * 128), o = tmem + COL_O + slot * 128;
+              const uint32_t acc = t >= AHEAD;
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            mma_ss(tmem + COL_S + slot * 128, desc_sw128(qs + (k >> 2) * ROWS * 128 + (k & 3) * 32, 16),
-                   desc_sw128(kb + (k >> 2) * KT * 128 + (k & 3) * 32, 16), QK, k > 0);
-        };
-        const auto pv = [&](int slot, uint32_t c, bool acc) {
-          if (!alive) return;
-          const uint32_t vb = ra + (c % NBUF) * BUF;
+              for (int k = 0; k < KT / 16; ++k) mma_ts(o, s_cols + k * 8, v + k * 128, PV, k ? 1u : acc, leader);
+            }
+            if (last) commit(&sh.empty[cv % NBUF], leader);
+            if (!PAIR) ++cnt;
+          }
+          if (more) {
+            const uint32_t c = PAIR ? ck : cnt;
+            if (first) wait(&sh.full[c % NBUF], (c / NBUF) & 1);
+            if (!alive) break;
+            if (!idle) {
+              const uint32_t q = qd + (PAIR ? slot * TILE * 8 : 0), kd = desc_lo(ring_at + (c % NBUF) * BUF, 16);
 #pragma unroll
-          for (int k = 0; k < KT / 16; ++k)
-            mma_ts(tmem + COL_O + slot * 128, tmem + COL_S + slot * 128 + k * 8, desc_sw128(vb + k * 2048, KT * 128), PV,
-                   acc || k > 0);
-        };
-        const auto commit = [&](uint64_t* bar) {
-          if (alive) mma_commit(smem_u32(bar));
-        };
-        const auto weights = [&](int slot) {
-          wait(&sh.p_ready[slot], np[slot]++ & 1);
-          fence_after_sync();
-        };
-        if (PAIR) {
-          buf_full(cnt);
-          qk(0, cnt);
-          commit(&sh.s_full[0]);
-          if (two) qk(1, cnt);
-          commit(&sh.s_full[1]);
-          commit(&sh.empty[cnt % NBUF]);
-          ++cnt;
-          for (int t = 0; t < n && alive; ++t) {
-            const bool more = t + 1 < n;
-            const uint32_t cv = cnt, ck = cnt + 1;
-            weights(0);
-            buf_full(cv);
-            pv(0, cv, t > 0);
-            if (more) buf_full(ck), qk(0, ck);
-            commit(&sh.s_full[0]);
-            if (two) weights(1), pv(1, cv, t > 0);
-            commit(&sh.empty[cv % NBUF]);
-            if (more) {
-              if (two) qk(1, ck);
-              commit(&sh.empty[ck % NBUF]);
+              for (int k = 0; k < DP / 16; ++k)
+                mma_ss(s_cols, q + (k >> 2) * ROWS * 8 + (k & 3) * 2, kd + (k >> 2) * KT * 8 + (k & 3) * 2, QK, k > 0, leader);
             }
-            if (two) commit(&sh.s_full[1]);
-            cnt += more ? 2 : 1;
+            if (last) commit(&sh.empty[c % NBUF], leader);
+            if (last && t + AHEAD == n - 1) commit(&sh.q_free, leader);
+            if (!PAIR) ++cnt;
           }
-        } else {
-          for (int t = 0; t < 2; ++t) {
-            if (t < n) {
-              buf_full(cnt);
-              qk(t, cnt);
-              commit(&sh.empty[cnt % NBUF]);
-              ++cnt;
-            }
-            commit(&sh.s_full[t]);
-          }
-          for (int t = 0; t < n && alive; ++t) {
-            const int slot = t & 1;
-            weights(slot);
-            buf_full(cnt);
-            pv(slot, cnt, t > 1);
-            commit(&sh.empty[cnt % NBUF]);
-            ++cnt;
-            if (t + 2 < n) {
-              buf_full(cnt);
-              qk(slot, cnt);
-              commit(&sh.empty[cnt % NBUF]);
-              ++cnt;
-            }
-            commit(&sh.s_full[slot]);
-          }
+          if (PAIR && slot == 1) cnt += (t >= 0) + more;
+          if (!idle || t < 0) commit(&sh.s_full[slot], leader);
         }
       }
       // what has been issued completes before the block frees its tensor memory
-      mma_commit(smem_u32(&sh.done));
+      commit(&sh.done, leader);
       mbar_wait(&sh.done, 0);
     }
     __syncwarp();
   } else {
     // ---- softmax slots
-    set_regs<192, true>();
+    set_regs<SLOT_REGS, true>();
     const int slot = warp >> 2, r = tid & (TILE - 1);
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_addr = lanes + COL_S + slot * 128, o_addr = lanes + COL_O + slot * 128;
-    const float alpha = fabsf(a.t.alpha);
-    const uint32_t flip = a.t.alpha < 0 ? 0x80008000u : 0u, keep = a.t.alpha == 0 ? 0u : 0xFFFFFFFFu;
-    const float scale_s = a.t.alpha == 0 ? 1.0f : alpha;
-    uint32_t ns = 0, first = 0;  // phases of s_full seen; ring position of the item's first tile
+    const float scale_s = a.t.alpha == 0 ? 1.0f : fabsf(a.t.alpha);
+    uint32_t ns = 0, first = 0, items = 0;  // phases of s_full seen; ring position of the item's first tile; items
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+      if (alive) alive = __all_sync(0xffffffffu, wait_phase(bar, parity));
     };
     while (pos < end) {
       const Item it = sch.item(a, pos, end);
@@ -429,28 +567,6 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
       const int rows = min(TILE, all_rows - (PAIR ? slot * TILE : 0));  // of this slot's tile; may be <= 0 for PAIR
       const int R = it.m * ROWS + (PAIR ? slot * TILE : 0) + min(r, max(rows, 1) - 1);
       const int tok = (int)div_by((uint32_t)R, a.by_group);
-      // the slot's query rows into shared memory (PAIR: its own tile; else half of the pieces each)
-      if (rows > 0) {
-        const T* q = (const T*)a.t.q + (int64_t)(it.q0 + tok) * a.t.q_stride +
-                     (int64_t)(it.h * a.group + R - tok * a.group) * a.t.q_head_stride;
-        constexpr int PIECES = PAIR ? DP / 8 : DP / 16;
-        const int p0 = PAIR ? 0 : slot * PIECES;
-        uint4 x[PIECES];
-#pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-          x[p] = (p0 + p) * 8 < a.t.d ? *(const uint4*)(q + (p0 + p) * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-          x[p].x = (x[p].x & keep) ^ flip, x[p].y = (x[p].y & keep) ^ flip;
-          x[p].z = (x[p].z & keep) ^ flip, x[p].w = (x[p].w & keep) ^ flip;
-          *(uint4*)(qbuf + tile_off((PAIR ? slot * TILE : 0) + r, p0 + p, ROWS)) = x[p];
-        }
-      }
-      if (r == 0) sh.dirty[slot] = 0;
-      fence_async_smem();
-      fence_before_sync();
-      arrive(&sh.q_full);
-
       const bool warp_rows = (r & ~31) < rows;
       const int tiles = PAIR ? (rows > 0 ? n : 0) : (n + 1 - slot) / 2;
       float m = -INFINITY, l = 0.0f;
@@ -462,61 +578,80 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
         const uint32_t* ok = sh.page_ok[(first / 2 + t) % PAGE_RING];
         const bool masked = key0 + KT > ctx || (ok[0] & ok[1] & ok[2] & ok[3]) != 0xFFFFFFFFu;
         if (warp_rows && alive) {
-          float s[KT];
-#pragma unroll
-          for (int c = 0; c < KT / 32; ++c) ld32(s_addr + c * 32, (uint32_t*)s + c * 32);
-          tmem_wait_ld();
+          uint32_t vis[KT / 32];
           if (masked) {
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c) {
-              const uint32_t vis = seen_word(a, it, tok, key0 + c * 32) & ok[c];
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((vis >> e) & 1)) s[c * 32 + e] = -INFINITY;
-            }
+            for (int c = 0; c < KT / 32; ++c) vis[c] = seen_word(a, it, tok, key0 + c * 32) & ok[c];
           }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          // One pass in the common case: the weights against the maximum so far, while the tile's own maximum is taken.
+          // They are stored, over the scores, only if no row's maximum grew by more than 8; else O is rescaled and
+          // a second pass computes them anew. A slot's first tile takes its maximum before.
+          uint32_t u[2][16], p[KT / 2];
+          float2 sum[2];
+          float mx[2] = {-INFINITY, -INFINITY};
+          // calls f(c, scores of columns 16 c ..), the next columns on their way
+          const auto columns = [&](auto f) {
+            ld16(s_addr, u[0]);
 #pragma unroll
-          for (int e = 0; e < KT; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_s;
-          const bool grow = top > m + 8.0f || (m == -INFINITY && top != -INFINITY);
-          if (__any_sync(0xffffffffu, grow)) {
+            for (int c = 0; c < KT / 16; ++c) {
+              uint32_t* v = u[c & 1];
+              wait_ld16(v);
+              if (c + 1 < KT / 16) ld16(s_addr + (c + 1) * 16, u[(c + 1) & 1]);
+              if (masked) hide16(v, vis[c >> 1] >> (c & 1) * 16);
+              f(c, v);
+            }
+          };
+          if (i == 0) {
+            columns([&](int, const uint32_t* v) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) mx[e & 1] = max3(mx[e & 1], __uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+            });
+            m = fmaxf(mx[0], mx[1]) * scale_s;
+          }
+          for (int pass = 0; pass < 2; ++pass) {
+            const float ref = m == -INFINITY ? 0.0f : m;
+            const float2 sc = make_float2(scale_s, scale_s), sub = make_float2(-ref, -ref);
+            mx[0] = mx[1] = -INFINITY;
+            sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+            columns([&](int c, const uint32_t* v) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                float2 x = make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+                mx[e & 1] = max3(mx[e & 1], x.x, x.y);
+                x = fma2(x, sc, sub);
+                x.x = ex2(x.x), x.y = ex2(x.y);
+                sum[e & 1] = add2(sum[e & 1], x);
+                p[c * 8 + e] = pack2(x.x, x.y, T());
+              }
+            });
+            const float top = fmaxf(mx[0], mx[1]) * scale_s;
+            const bool grow = top > m + 8.0f || (m == -INFINITY && top != -INFINITY);
+            if (!__any_sync(0xffffffffu, grow)) break;
             const float f = grow ? (m == -INFINITY ? 0.0f : ex2(m - top)) : 1.0f;
             if (grow) m = top;
             l *= f;
             if (i > 0) {
+#pragma unroll 1
+              for (int c = 0; c < DP / 16; ++c) {
+                uint32_t o[16];
+                ld16(o_addr + c * 16, o);
+                wait_ld16(o);
 #pragma unroll
-              for (int c = 0; c < DP / 32; ++c) {
-                uint32_t o[32];
-                ld32(o_addr + c * 32, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                st32(o_addr + c * 32, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                st16(o_addr + c * 16, o);
               }
             }
           }
-          const float ref = m == -INFINITY ? 0.0f : m;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t p[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float x = ex2(fmaf(s[c * 64 + 2 * e], scale_s, -ref)), y = ex2(fmaf(s[c * 64 + 2 * e + 1], scale_s, -ref));
-              sum[e & 1] += x, sum[2 + (e & 1)] += y;
-              p[e] = pack2(x, y, T());
-            }
-            st32(s_addr + c * 32, p);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          st32(s_addr, p);
+          st32(s_addr + 32, p + 32);
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
         }
         // drafted keys: their infinities and NaN may not meet the zero weight of a row that does not see them
         if (key0 + KT > ctx && (!PAIR || slot == 0)) {
           const uint32_t c = first + (PAIR ? 1 + 2 * t : n == 1 ? 1 : 2 + t + min(t, n - 2));
           wait(&sh.full[c % NBUF], (c / NBUF) & 1);
-          if (alive && clean_row<T, DP>(ring + (c % NBUF) * BUF, r) && key0 + r < it.len) sh.dirty[slot] = 1;
+          if (alive && clean_row<T, DP>(ring + (c % NBUF) * BUF, r) && key0 + r < it.len) sh.dirty[items & 1][slot] = 1;
           fence_async_smem();
         }
         fence_before_sync();
@@ -524,6 +659,7 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
       }
       wait(&sh.s_full[slot], ns++ & 1);  // the slot's products are done
       fence_after_sync();
+      arrive(&sh.seen);
       first += 2 * n;
 
       // join the slots (PAIR: each has rows of its own) and write the rows
@@ -537,7 +673,9 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
       } else {
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      const bool dirty = sh.dirty[0] || sh.dirty[1];
+      const bool dirty = sh.dirty[items & 1][0] || sh.dirty[items & 1][1];
+      ++items;
+      if (r == 0) sh.dirty[items & 1][slot] = 0;
       const float mm = fmaxf(ml[0], ml[1]), ref = mm == -INFINITY ? 0.0f : mm;
       const float f0 = exp2f(ml[0] - ref), f1 = PAIR || n < 2 ? 0.0f : exp2f(ml[1] - ref);
       const float lsum = ll[0] * f0 + ll[1] * (PAIR ? 0.0f : exp2f(ml[1] - ref));
@@ -564,7 +702,13 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
             for (int e = 0; e < 32; ++e) o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
           }
           const int ch = c0 + c * 32;
-          if (mine && dirty) add_not_finite<T, 32>(a, it, tok, it.kt0 * KT, it.kt1 * KT, ch, o);
+          if (mine && dirty) {
+            float extra[32];
+            for (int e = 0; e < 32; ++e) extra[e] = 0.0f;
+            add_not_finite<T, 32>(a, it, tok, it.kt0 * KT, it.kt1 * KT, ch, extra);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] += extra[e];
+          }
           if (mine && whole) {
             T* dst = (T*)a.t.out + head * a.t.d + ch;
 #pragma unroll
@@ -578,7 +722,7 @@ __global__ void __launch_bounds__(THREADS, 1) many_rows_kernel(Args a) {
           } else if (mine) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              *(float4*)(part + (int64_t)pr * DP + ch + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              *(float4*)(part + ((ch + e) * ROWS + pr * 4)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
           __syncwarp();
         }
