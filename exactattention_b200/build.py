@@ -92,7 +92,8 @@ def build_serving_native(force: bool = False) -> str:
         lib = cpp_extension.library_paths()
         subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-I{p}" for p in inc], "-o", SERVING_NATIVE + ".tmp",
                         src, *[f"-L{p}" for p in lib], f"-L{HERE}", "-l:libexactattn_cuda.so", "-lc10", "-lc10_cuda",
-                        "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], check=True)
+                        "-ltorch_cpu",
+                        "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], check=True)
         os.replace(SERVING_NATIVE + ".tmp", SERVING_NATIVE)
     return SERVING_NATIVE
 

@@ -1,25 +1,35 @@
 // Penalties for repeated tokens, biases and grammar masks on logits (ea_process_logits_cuda).
 //
-// Bound by HBM: a row's logits are read once and written once. Two kernels:
-//   dense_kernel   streams every row through, setting what its grammar mask forbids to -inf;
-//   sparse_kernel  a block a row: collects the tokens that penalties or biases change in a hash table in shared
-//                  memory and corrects those tokens of the output. Its table is built while the dense kernel drains
-//                  (programmatic dependent launch); only the corrections wait for it.
-// One kernel with a table of counts beside each chunk of the vocabulary was measured first: 68 us against 35 us for
-// 256 rows of 131072 16-bit logits with 4096 history entries, because every chunk scans the whole history and lanes
-// with and without a token take turns.
-// A table entry's word: bits 0-19 how often the token was generated, bits 20-30 which bias entry it has first
-// (EA_LOGITS_MAX_BIASES - entry, 0: none), bit 31 whether the prompt holds it. The words are integers, so the order of
-// the atomics cannot change them.
+// Bound by HBM: a row's logits are read once and written once; what the grammar mask forbids becomes -inf on the way, and
+// the few tokens that penalties or biases change are corrected afterwards. Which these are is kept in 32-bit words:
+//   bits 0-19 how often the token was generated, bits 20-30 which bias entry it has first
+//   (EA_LOGITS_MAX_BIASES - entry, 0: none), bit 31 whether the prompt holds it.
+// The words are integers, so the order of the atomics cannot change them. Whoever finds a word (or a table entry) fresh
+// puts it on a list, from which the corrections are done with full warps.
+//   Many rows: dense_kernel streams all rows through; sparse_kernel, a block a row, collects the row's history, path and
+//   biases in a hash table in shared memory and corrects their tokens. It is launched to start while the dense kernel
+//   drains; only its stores wait for it.
+//   Few rows (a block or two for every SM): chunk_kernel alone, with a word for every token of its chunk of the row's
+//   vocabulary; every chunk reads the whole history, which is cheaper than a second launch (6 us against 13 us for one
+//   row of 32000 tokens).
+// Measured otherwise for 256 rows of 131072 16-bit logits with 4096 history entries: the chunk kernel for all 68 us; with
+// a cluster of blocks sharing the scan through distributed shared memory 99 us; with a kernel before it that sorts
+// every row's history by chunk 60 us.
+#include <type_traits>
+
 #include "ea_serving.cuh"
 
 namespace ea {
 namespace serving {
 namespace {
 
-constexpr int DENSE_THREADS = 256, UNROLL = 4;  // 16-byte pieces a thread has in flight
-constexpr int SPARSE_THREADS = 512, BATCH = 8;  // entries a thread works on at a time
-constexpr int MAX_SLOTS = 16384, FILL = 12288;  // table entries, and how many tokens one pass puts into them
+constexpr int THREADS = 512;        // of the chunk and the sparse kernel
+constexpr int DENSE_THREADS = 256;
+constexpr int UNROLL = 4;           // 16-byte pieces a thread has in flight
+constexpr int BATCH = 8;            // history entries a thread asks for at a time
+constexpr int LIST = 4096;          // tokens a chunk lists; more: its table is searched
+constexpr int MAX_CHUNK = 16384 + 16;
+constexpr int MAX_SLOTS = 16384;    // entries of a hash table
 constexpr uint32_t COUNT = 0xFFFFFu, PROMPT = 0x80000000u;
 constexpr int CODE_SHIFT = 20;
 
@@ -28,32 +38,118 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-// The row's mask bits, nullptr where every token is allowed.
-__device__ __forceinline__ const uint32_t* mask_of(const ea_process_logits_t& a, int64_t row) {
-  if (!a.allowed_bits) return nullptr;
-  const int b = a.row_seq ? a.row_seq[row] : (int)row;
-  const int m = a.mask_rows ? a.mask_rows[row] : (int)row;
-  return b >= 0 && b < a.batch && m >= 0 && m < a.num_masks ? (const uint32_t*)a.allowed_bits + m * a.mask_stride : nullptr;
+// -inf in the elements whose bit of `no` is set
+template <typename T, int VEC>
+__device__ __forceinline__ void forbid(Pack<T, VEC>& p, uint32_t no) {
+  if constexpr (sizeof(T) == 2 && VEC == 8) {
+    constexpr uint32_t INF2 = std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+    uint32_t* w = (uint32_t*)&p;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // four bits to four bytes of 0 or 255, then every byte twice
+      const uint32_t b = (((no >> 4 * h & 15u) * 0x00204081u) & 0x01010101u) * 255u;
+      const uint32_t m0 = __byte_perm(b, 0, 0x1100), m1 = __byte_perm(b, 0, 0x3322);
+      w[2 * h] = (w[2 * h] & ~m0) | (INF2 & m0);
+      w[2 * h + 1] = (w[2 * h + 1] & ~m1) | (INF2 & m1);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if ((no >> e) & 1) p.v[e] = from_f<T>(-INFINITY);
+  }
 }
 
-// Thread `tid` of `threads` streams pieces tid, tid + threads, .. (UNROLL of them) of a row from piece `first` on.
+// A row's sequence and lists.
+struct Row {
+  int b, n_hist, n_prompt, n_path;
+  bool counts;  // history and path matter
+  float rep, freq, pres;
+  const int32_t *hist, *path;
+  const uint32_t* seen;  // path members, nullptr: all
+};
+__device__ __forceinline__ Row row_of(const ea_process_logits_t& a, int64_t row) {
+  Row r;
+  const int b = a.row_seq ? a.row_seq[row] : (int)row;
+  r.b = b >= 0 && b < a.batch ? b : -1;
+  r.rep = r.b >= 0 && a.repetition ? a.repetition[b] : 1.0f;
+  r.freq = r.b >= 0 && a.frequency ? a.frequency[b] : 0.0f;
+  r.pres = r.b >= 0 && a.presence ? a.presence[b] : 0.0f;
+  r.counts = r.b >= 0 && (r.rep != 1.0f || r.freq != 0.0f || r.pres != 0.0f) && (a.history || a.draft_tokens);
+  r.n_hist = r.n_prompt = r.n_path = 0;
+  r.hist = r.path = nullptr, r.seen = nullptr;
+  if (!r.counts) return r;
+  if (a.history) {
+    r.hist = a.history + (int64_t)b * a.history_stride;
+    r.n_hist = min(max(a.history_lens[b], 0), a.max_history);
+    r.n_prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), r.n_hist) : 0;
+  }
+  if (a.draft_tokens) {
+    const int64_t q0 = a.q_start[b], q1 = min((int64_t)a.q_start[b + 1], a.rows);
+    if (q0 >= 0 && q0 < q1) {
+      const int64_t most = a.tree_mask ? (int64_t)a.tree_words * 32 : row - q0 + 1;
+      r.n_path = (int)max(min(min(q1 - q0, (int64_t)EA_LOGITS_MAX_PATH), most), (int64_t)0);
+      r.path = a.draft_tokens + q0;
+      if (a.tree_mask) r.seen = (const uint32_t*)a.tree_mask + row * a.tree_words;
+    }
+  }
+  return r;
+}
+// Token j of the lists: history, then path; EMPTY where there is none or the path leaves it out.
+constexpr uint32_t EMPTY = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t token_of(const Row& r, int j) {
+  if (j < r.n_hist) return (uint32_t)r.hist[j];
+  j -= r.n_hist;
+  if (j >= r.n_path || (r.seen && !((r.seen[j >> 5] >> (j & 31)) & 1))) return EMPTY;
+  return (uint32_t)r.path[j];
+}
 template <typename T, int VEC>
-__device__ __forceinline__ void stream_row(const ea_process_logits_t& a, int64_t row, const uint32_t* bits, int first, int tid,
-                                           int threads) {
+__device__ __forceinline__ int misalignment(const ea_process_logits_t& a, int64_t row) {
+  return (int)(((uintptr_t)((const T*)a.logits + row * a.logits_stride) / sizeof(T)) % VEC);
+}
+
+// The row's mask bits, nullptr where every token is allowed.
+__device__ __forceinline__ const uint32_t* mask_of(const ea_process_logits_t& a, int64_t row, bool real) {
+  const int m = a.allowed_bits && real ? (a.mask_rows ? a.mask_rows[row] : (int)row) : -1;
+  return m >= 0 && m < a.num_masks ? (const uint32_t*)a.allowed_bits + m * a.mask_stride : nullptr;
+}
+// The logit of a token whose word is not zero.
+__device__ __forceinline__ float adjust(float x, uint32_t w, uint32_t token, const Row& r, const int32_t* ids, const float* vals,
+                                        int n_bias, bool dup) {
+  const uint32_t cnt = w & COUNT, code = (w >> CODE_SHIFT) & 0x7FFu;
+  if (cnt || (w & PROMPT)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
+  x = __fsub_rn(x, __fmul_rn(r.freq, (float)cnt));
+  if (cnt) x = __fsub_rn(x, r.pres);
+  if (code) {
+    int e = EA_LOGITS_MAX_BIASES - (int)code;
+    x = __fadd_rn(x, vals[e]);
+    if (dup)
+      for (++e; e < n_bias; ++e)
+        if ((uint32_t)ids[e] == token) x = __fadd_rn(x, vals[e]);
+  }
+  return x;
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(DENSE_THREADS) dense_kernel(ea_process_logits_t a, int chunks, FastDiv by_chunks) {
   using P = Pack<T, VEC>;
+  cudaTriggerProgrammaticLaunchCompletion();
+  const int64_t row = div_by(blockIdx.x, by_chunks);
+  const int part = (int)(blockIdx.x - row * chunks);
   const T* src = (const T*)a.logits + row * a.logits_stride;
   T* dst = (T*)a.out + row * a.out_stride;
   // Pieces are aligned in memory, so the row's first one may begin before its first token.
-  const int v0 = (first + tid) * VEC - (int)(((uintptr_t)src / sizeof(T)) % VEC);
+  const int v0 = (part * UNROLL * DENSE_THREADS + (int)threadIdx.x) * VEC - misalignment<T, VEC>(a, row);
   P x[UNROLL];
 #pragma unroll
   for (int j = 0; j < UNROLL; ++j) {
-    const int v = v0 + j * threads * VEC;
+    const int v = v0 + j * DENSE_THREADS * VEC;
     if (v >= 0 && v + VEC <= a.vocab) x[j] = *(const P*)(src + v);
   }
+  const int b = a.row_seq ? a.row_seq[row] : (int)row;
+  const uint32_t* bits = mask_of(a, row, b >= 0 && b < a.batch);
 #pragma unroll
   for (int j = 0; j < UNROLL; ++j) {
-    const int v = v0 + j * threads * VEC;
+    const int v = v0 + j * DENSE_THREADS * VEC;
     if (v >= a.vocab || v + VEC <= 0) continue;
     const bool whole = v >= 0 && v + VEC <= a.vocab;
     if (!whole) {
@@ -62,12 +158,9 @@ __device__ __forceinline__ void stream_row(const ea_process_logits_t& a, int64_t
         if (v + e >= 0 && v + e < a.vocab) x[j].v[e] = src[v + e];
     }
     if (bits) {
-      // bit e of `no`: token v + e is forbidden; the piece may lie in two words
+      // bit e: token v + e is allowed; the piece may lie in two words
       const int lo = max(v, 0), hi = min(v + VEC, a.vocab) - 1;
-      const uint32_t no = ~__funnelshift_r(bits[lo >> 5], bits[hi >> 5], lo & 31) << (lo - v);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if ((no >> e) & 1) x[j].v[e] = from_f<T>(-INFINITY);
+      forbid<T, VEC>(x[j], ~__funnelshift_r(bits[lo >> 5], bits[hi >> 5], lo & 31) << (lo - v));
     }
     if (whole) {
       *(P*)(dst + v) = x[j];
@@ -79,185 +172,268 @@ __device__ __forceinline__ void stream_row(const ea_process_logits_t& a, int64_t
   }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(DENSE_THREADS) dense_kernel(ea_process_logits_t a, FastDiv by_chunks, int chunks) {
-  cudaTriggerProgrammaticLaunchCompletion();
-  const int64_t row = div_by(blockIdx.x, by_chunks);
-  const int part = (int)(blockIdx.x - row * chunks);
-  stream_row<T, VEC>(a, row, mask_of(a, row), part * UNROLL * DENSE_THREADS, threadIdx.x, DENSE_THREADS);
-}
-
-// VEC 0: the dense kernel has written the rows; else this block streams its row itself.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(SPARSE_THREADS) sparse_kernel(ea_process_logits_t a, int slots, int shift) {
-  extern __shared__ uint32_t keys[];  // token + 1, 0: free; then the words
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t a, int slots, int shift) {
+  extern __shared__ uint32_t keys[];  // token + 1, 0: free; then the words, then the list of used entries
   uint32_t* words = keys + slots;
-  __shared__ int dup;
+  uint16_t* list = (uint16_t*)(words + slots);
+  __shared__ int dup, listed;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
-  const int b = a.row_seq ? a.row_seq[row] : (int)row;
-  const bool real = b >= 0 && b < a.batch;
-  // the first history entries, asked for before their number is known
-  const int32_t* hist = a.history ? a.history + (int64_t)(real ? b : 0) * a.history_stride : nullptr;
-  uint32_t tok[BATCH];
-  const auto fetch = [&](int first, int n) {
-#pragma unroll
-    for (int e = 0; e < BATCH; ++e) {
-      const int i = first + e * SPARSE_THREADS + tid;
-      tok[e] = i < n ? (uint32_t)hist[i] : 0xFFFFFFFFu;
-    }
-  };
-  if (real && hist) fetch(0, a.max_history);
-  const uint32_t* bits = mask_of(a, row);
-  const float rep = real && a.repetition ? a.repetition[b] : 1.0f, freq = real && a.frequency ? a.frequency[b] : 0.0f,
-              pres = real && a.presence ? a.presence[b] : 0.0f;
-  const bool counts = rep != 1.0f || freq != 0.0f || pres != 0.0f;
-  // the lists: history, path (drafted tokens), biases
-  const int n_hist = counts && hist ? min(max(a.history_lens[b], 0), a.max_history) : 0;
-  const int n_prompt = n_hist && a.prompt_lens ? min(max(a.prompt_lens[b], 0), n_hist) : 0;
-  int n_path = 0;
-  const int32_t* path = nullptr;
-  if (counts && a.draft_tokens) {
-    const int64_t q0 = a.q_start[b], q1 = min((int64_t)a.q_start[b + 1], a.rows);
-    if (q0 >= 0 && q0 < q1) {
-      n_path = (int)max(min(min(q1 - q0, (int64_t)EA_LOGITS_MAX_PATH), a.tree_mask ? (int64_t)a.tree_words * 32 : row - q0 + 1), (int64_t)0);
-      path = a.draft_tokens + q0;
-    }
-  }
-  const uint32_t* seen = a.tree_mask ? (const uint32_t*)a.tree_mask + row * a.tree_words : nullptr;
-  const int n_bias = real ? a.num_biases : 0;
-  const int32_t* ids = a.bias_ids + (int64_t)b * n_bias;
-  const float* vals = a.bias_values + (int64_t)b * n_bias;
-  const int64_t all = (int64_t)n_hist + n_path + n_bias;
-  if (VEC == 0 && all == 0) {
+  const Row r = row_of(a, row);
+  const uint32_t* bits = mask_of(a, row, r.b >= 0);
+  const int n_bias = r.b >= 0 ? a.num_biases : 0, n = r.n_hist + r.n_path;
+  const int32_t* ids = a.bias_ids + (int64_t)r.b * n_bias;
+  const float* vals = a.bias_values + (int64_t)r.b * n_bias;
+  const T* src = (const T*)a.logits + row * a.logits_stride;
+  T* dst = (T*)a.out + row * a.out_stride;
+  const uint32_t vocab = (uint32_t)a.vocab;
+  if (n + n_bias == 0) {
     cudaGridDependencySynchronize();  // nothing after this kernel may overtake the dense one
     return;
   }
   // One pass where the lists fit; else as many as the vocabulary needs, pass p taking the tokens that are p modulo
   // their number, so that no pass can overfill the table.
-  const uint32_t vocab = (uint32_t)a.vocab, passes = all <= slots / 4 * 3 ? 1u : (vocab + FILL - 1) / FILL;
-  const auto slot_of = [&](uint32_t t) -> uint32_t* {
-    for (uint32_t h = (t * 2654435761u) >> shift;; h = (h + 1) & (uint32_t)(slots - 1)) {
+  const uint32_t fill = slots / 4 * 3, passes = n + n_bias <= (int)fill ? 1u : (vocab + fill - 1) / fill;
+  // The word of token t. The table never fills up; the bound on the search is for safety.
+  const auto word_of = [&](uint32_t t) -> uint32_t* {
+    uint32_t h = (t * 2654435761u) >> shift;
+    for (int i = 0; i < slots; ++i, h = (h + 1) & (uint32_t)(slots - 1)) {
       uint32_t k = keys[h];
-      if (k == 0) k = atomicCAS(keys + h, 0u, t + 1);
-      if (k == 0 || k == t + 1) return words + h;
+      if (k == 0) {
+        k = atomicCAS(keys + h, 0u, t + 1);
+        if (k == 0) {
+          list[atomicAdd(&listed, 1)] = (uint16_t)h;
+          break;
+        }
+      }
+      if (k == t + 1) break;
     }
+    return words + h;
   };
   for (uint32_t pass = 0; pass < passes; ++pass) {
     const auto mine = [&](uint32_t t) { return t < vocab && (passes == 1 || t % passes == pass); };
-    for (int i = tid; i < slots / 2; i += SPARSE_THREADS) ((uint4*)keys)[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) dup = 0;
+    for (int i = tid; i < slots / 2; i += THREADS) ((uint4*)keys)[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) dup = listed = 0;
+    uint32_t tok[BATCH];
+#pragma unroll
+    for (int e = 0; e < BATCH; ++e) tok[e] = token_of(r, e * THREADS + tid);
     __syncthreads();
-    for (int first = 0; first < n_hist; first += BATCH * SPARSE_THREADS) {
-      if (first || pass) fetch(first, n_hist);
+    for (int first = 0; first < n; first += BATCH * THREADS) {
+      if (first) {
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) tok[e] = token_of(r, first + e * THREADS + tid);
+      }
 #pragma unroll
       for (int e = 0; e < BATCH; ++e) {
-        const int i = first + e * SPARSE_THREADS + tid;
-        if (i >= n_hist || !mine(tok[e])) continue;
-        if (i < n_prompt) atomicOr(slot_of(tok[e]), PROMPT);
-        else atomicAdd(slot_of(tok[e]), 1u);
+        if (!mine(tok[e])) continue;
+        uint32_t* w = word_of(tok[e]);
+        if (first + e * THREADS + tid < r.n_prompt) atomicOr(w, PROMPT);
+        else atomicAdd(w, 1u);
       }
     }
-    for (int j = tid; j < n_path; j += SPARSE_THREADS) {
-      if (seen && !((seen[j >> 5] >> (j & 31)) & 1)) continue;
-      const uint32_t t = (uint32_t)path[j];
-      if (mine(t)) atomicAdd(slot_of(t), 1u);
-    }
     __syncthreads();
-    for (int e = tid; e < n_bias; e += SPARSE_THREADS) {
+    for (int e = tid; e < n_bias; e += THREADS) {
       const uint32_t t = (uint32_t)ids[e];
       if (!mine(t)) continue;
-      uint32_t* w = slot_of(t);
+      uint32_t* w = word_of(t);
       const uint32_t old = atomicMax(w, (*w & (PROMPT | COUNT)) | (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT);
       if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
     }
     __syncthreads();
-    // values and mask words of up to BATCH entries a thread at a time
-    for (int i0 = tid; i0 < slots; i0 += BATCH * SPARSE_THREADS) {
+    const int used = listed;
+    for (int first = 0; first < used; first += BATCH * THREADS) {
       T old[BATCH];
-      uint32_t mask[BATCH];
+      uint32_t ok = 0;
 #pragma unroll
       for (int e = 0; e < BATCH; ++e) {
-        const int i = i0 + e * SPARSE_THREADS;
-        tok[e] = i < slots ? keys[i] : 0;
-        mask[e] = 0xFFFFFFFFu;
-        if (tok[e]) {
-          const uint32_t t = tok[e] - 1;
-          old[e] = ((const T*)a.logits)[row * a.logits_stride + t];
-          if (bits) mask[e] = bits[t >> 5];
+        const int i = first + e * THREADS + tid;
+        tok[e] = i < used ? list[i] : 0;
+        if (i < used) {
+          const uint32_t t = keys[tok[e]] - 1;
+          old[e] = src[t];
+          ok |= (bits ? (bits[t >> 5] >> (t & 31)) & 1u : 1u) << e;
         }
       }
-      if (pass == 0 && i0 == tid) {  // the row is written
-        if constexpr (VEC == 0) cudaGridDependencySynchronize();
-        else {
-          const int pieces = (int)((vocab + 2 * VEC - 2) / VEC);
-          for (int first = 0; first < pieces; first += UNROLL * SPARSE_THREADS)
-            stream_row<T, VEC>(a, row, bits, first, tid, SPARSE_THREADS);
-          __syncthreads();
-        }
-      }
+      if (pass == 0 && first == 0) cudaGridDependencySynchronize();  // the dense kernel's rows are written
 #pragma unroll
       for (int e = 0; e < BATCH; ++e) {
-        const uint32_t t = tok[e] - 1;
-        if (!tok[e] || !((mask[e] >> (t & 31)) & 1)) continue;
-        const uint32_t w = words[i0 + e * SPARSE_THREADS], cnt = w & COUNT, code = (w >> CODE_SHIFT) & 0x7FFu;
-        float x = to_f(old[e]);
-        if (cnt || (w & PROMPT)) x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-        x = __fsub_rn(x, __fmul_rn(freq, (float)cnt));
-        if (cnt) x = __fsub_rn(x, pres);
-        if (code) {
-          int f = EA_LOGITS_MAX_BIASES - (int)code;
-          x = __fadd_rn(x, vals[f]);
-          if (dup)
-            for (++f; f < n_bias; ++f)
-              if ((uint32_t)ids[f] == t) x = __fadd_rn(x, vals[f]);
-        }
-        ((T*)a.out)[row * a.out_stride + t] = from_f<T>(x);
+        if (!((ok >> e) & 1)) continue;
+        const uint32_t t = keys[tok[e]] - 1;
+        dst[t] = from_f<T>(adjust(to_f(old[e]), words[tok[e]], t, r, ids, vals, n_bias, dup != 0));
       }
     }
+    if (pass == 0 && used == 0) cudaGridDependencySynchronize();
     __syncthreads();
   }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(THREADS, 2) chunk_kernel(ea_process_logits_t a, int chunk, int chunks, FastDiv by_chunks) {
+  using P = Pack<T, VEC>;
+  extern __shared__ uint4 table4[];
+  uint32_t* table = (uint32_t*)table4;
+  __shared__ uint16_t list[LIST];
+  __shared__ int dup, listed;
+  const int tid = threadIdx.x;
+  const int64_t row = div_by(blockIdx.x, by_chunks);
+  const int part = (int)(blockIdx.x - row * chunks);
+  const T* src = (const T*)a.logits + row * a.logits_stride;
+  T* dst = (T*)a.out + row * a.out_stride;
+  // Pieces are aligned in memory: place i of the chunk is token v0 + i, and the row's first piece may begin before its
+  // first token.
+  const int v0 = part * chunk - misalignment<T, VEC>(a, row);
+
+  P x[UNROLL];
+#pragma unroll
+  for (int j = 0; j < UNROLL; ++j) {
+    const int i = (j * THREADS + tid) * VEC, v = v0 + i;
+    if (i < chunk && v >= 0 && v + VEC <= a.vocab) x[j] = *(const P*)(src + v);
+  }
+
+  const Row r = row_of(a, row);
+  const uint32_t* bits = mask_of(a, row, r.b >= 0);
+  const int n_bias = r.b >= 0 ? a.num_biases : 0;
+  const bool tabled = r.counts || n_bias > 0;
+  const int32_t* ids = a.bias_ids + (int64_t)r.b * n_bias;
+  const float* vals = a.bias_values + (int64_t)r.b * n_bias;
+  uint32_t id = tid < n_bias ? (uint32_t)ids[tid] : EMPTY;
+  if (tabled) {
+    for (int i = tid; i < chunk / 4; i += THREADS) table4[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) dup = listed = 0;
+    __syncthreads();
+  }
+  // Puts a token on the list if its word was zero before.
+  const auto touch = [&](uint32_t at, uint32_t before) {
+    if (before) return;
+    const int k = atomicAdd(&listed, 1);
+    if (k < LIST) list[k] = (uint16_t)at;
+  };
+  if (r.counts) {
+    const int n = r.n_hist + r.n_path;
+#pragma unroll 4
+    for (int j = tid; j < n; j += THREADS) {
+      const uint32_t t = token_of(r, j), at = t - (uint32_t)v0;
+      if (t < (uint32_t)a.vocab && at < (uint32_t)chunk)
+        touch(at, j < r.n_prompt ? atomicOr(table + at, PROMPT) : atomicAdd(table + at, 1u));
+    }
+  }
+  if (n_bias) {
+    __syncthreads();  // the counts are complete
+    for (int e = tid; e < n_bias; e += THREADS) {
+      if (e != tid) id = (uint32_t)ids[e];
+      const uint32_t t = id, at = t - (uint32_t)v0;
+      if (t >= (uint32_t)a.vocab || at >= (uint32_t)chunk) continue;
+      const uint32_t old = atomicMax(table + at, (table[at] & (PROMPT | COUNT)) | (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT);
+      if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
+      touch(at, old);
+    }
+  }
+
+  for (int i0 = 0; i0 < chunk; i0 += UNROLL * THREADS * VEC) {
+    if (i0) {
+#pragma unroll
+      for (int j = 0; j < UNROLL; ++j) {
+        const int i = i0 + (j * THREADS + tid) * VEC, v = v0 + i;
+        if (i < chunk && v >= 0 && v + VEC <= a.vocab) x[j] = *(const P*)(src + v);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      const int i = i0 + (j * THREADS + tid) * VEC, v = v0 + i;
+      if (i >= chunk || v >= a.vocab || v + VEC <= 0) continue;
+      const bool whole = v >= 0 && v + VEC <= a.vocab;
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (v + e >= 0 && v + e < a.vocab) x[j].v[e] = src[v + e];
+      }
+      if (bits) {
+        // bit e: token v + e is allowed; the piece may lie in two words
+        const int lo = max(v, 0), hi = min(v + VEC, a.vocab) - 1;
+        forbid<T, VEC>(x[j], ~__funnelshift_r(bits[lo >> 5], bits[hi >> 5], lo & 31) << (lo - v));
+      }
+      if (whole) {
+        *(P*)(dst + v) = x[j];
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (v + e >= 0 && v + e < a.vocab) dst[v + e] = x[j].v[e];
+      }
+    }
+  }
+  if (!tabled) return;
+
+  __syncthreads();  // the chunk is written, the table and its list are complete
+  const bool search = listed > LIST;
+  const int n = search ? chunk : listed;
+  for (int i = tid; i < n; i += THREADS) {
+    const int at = search ? i : list[i], v = v0 + at;
+    const uint32_t w = table[at];
+    if (!w || (bits && !((bits[v >> 5] >> (v & 31)) & 1))) continue;
+    dst[v] = from_f<T>(adjust(to_f(src[v]), w, (uint32_t)v, r, ids, vals, n_bias, dup != 0));
+  }
+}
+
+int vec_of(const ea_process_logits_t& a) {
+  const int size = a.dtype == EA_FP32 ? 4 : 2, vec = 16 / size;
+  // 16-byte pieces where input and output rows are equally far from a 16-byte boundary
+  const bool same = ((uintptr_t)a.logits - (uintptr_t)a.out) % 16 == 0 &&
+                    (a.rows <= 1 || (a.logits_stride - a.out_stride) % vec == 0);
+  return same ? vec : 1;
+}
+
+// Room for `bytes` of dynamic shared memory, once per kernel and device.
+template <auto kernel>
+cudaError_t allow_smem(int bytes) {
+  static bool ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && ready[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) ready[dev] = true;
+  return e;
 }
 
 template <typename T, int VEC>
 int launch(const ea_process_logits_t& a, cudaStream_t st) {
   const bool counts = (a.repetition || a.frequency || a.presence) && (a.history || a.draft_tokens);
   const bool sparse = counts || a.num_biases, dense = a.allowed_bits || a.out != a.logits;
-  // Few short rows: a block that streams its row before it corrects it saves the second launch (6 us against 9 us for one
-  // row of 32000 tokens).
-  const bool together = sparse && dense && a.rows <= sm_count() && a.vocab <= 3 * UNROLL * SPARSE_THREADS * VEC;
-  if (dense && !together) {
+  // a row's places: its tokens, and those before it in its first 16-byte piece
+  const bool aligned = (uintptr_t)a.logits % 16 == 0 && (a.rows <= 1 || a.logits_stride * sizeof(T) % 16 == 0);
+  const int64_t places = (int64_t)a.vocab + (aligned ? 0 : VEC - 1);
+  cudaError_t e;
+  int chunk = 16384;
+  while (chunk > 2048 && a.rows * ((places + chunk - 1) / chunk) < 2 * sm_count()) chunk >>= 1;
+  int64_t chunks = (places + chunk - 1) / chunk;
+  if (sparse && a.rows * chunks <= 4 * sm_count()) {
+    chunk = (int)(((places + chunks - 1) / chunks + 15) & ~15ll);
+    if ((e = allow_smem<chunk_kernel<T, VEC>>(4 * MAX_CHUNK)) != cudaSuccess) return cuda_rc(e);
+    chunk_kernel<T, VEC><<<(unsigned)(a.rows * chunks), THREADS, 4 * (size_t)chunk, st>>>(a, chunk, (int)chunks, fast_div((uint32_t)chunks));
+    return cuda_rc(cudaGetLastError());
+  }
+  if (dense) {
     const int per_block = UNROLL * DENSE_THREADS * VEC;
-    const int chunks = (int)(((int64_t)a.vocab + VEC - 1 + per_block - 1) / per_block);
-    const int64_t blocks = a.rows * chunks;
-    if (blocks >= (1ll << 31)) return fail(-1, "process_logits: too many rows");
-    dense_kernel<T, VEC><<<(unsigned)blocks, DENSE_THREADS, 0, st>>>(a, fast_div((uint32_t)chunks), chunks);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_rc(e);
+    chunks = (places + per_block - 1) / per_block;
+    if (a.rows * chunks >= (1ll << 31)) return fail(-1, "process_logits: too many rows");
+    dense_kernel<T, VEC><<<(unsigned)(a.rows * chunks), DENSE_THREADS, 0, st>>>(a, (int)chunks, fast_div((uint32_t)chunks));
+    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_rc(e);
   }
   if (!sparse) return 0;
+  if (a.rows >= (1ll << 31)) return fail(-1, "process_logits: too many rows");
   // table: four thirds of the longest lists the sizes allow, at most MAX_SLOTS (then several passes)
   const int64_t longest = (int64_t)a.max_history + a.num_biases + (a.draft_tokens ? (a.tree_mask ? a.tree_words * 32 : 1024) : 0);
   int log2 = 10;
   while ((1 << log2) < MAX_SLOTS && (1 << log2) / 4 * 3 < longest) ++log2;
-  const int slots = 1 << log2;
-  const auto kernel = together ? sparse_kernel<T, VEC> : sparse_kernel<T, 0>;
-  static bool ready[2][64];  // per device
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev >= 64 || !ready[together][dev])) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SLOTS * 8);
-    if (e == cudaSuccess && dev < 64) ready[together][dev] = true;
-  }
-  if (e != cudaSuccess) return cuda_rc(e);
+  if ((e = allow_smem<sparse_kernel<T>>(MAX_SLOTS * 10)) != cudaSuccess) return cuda_rc(e);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.rows), cfg.blockDim = dim3(SPARSE_THREADS), cfg.dynamicSmemBytes = (size_t)slots * 8;
+  cfg.gridDim = dim3((unsigned)a.rows), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = (size_t)10 << log2;
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr, cfg.numAttrs = dense && !together ? 1 : 0;  // after the dense kernel only
-  e = cudaLaunchKernelEx(&cfg, kernel, a, slots, 32 - log2);
+  cfg.attrs = &attr, cfg.numAttrs = dense ? 1 : 0;  // after the dense kernel only
+  e = cudaLaunchKernelEx(&cfg, sparse_kernel<T>, a, 1 << log2, 32 - log2);
   if (e == cudaSuccess) e = cudaGetLastError();
   return cuda_rc(e);
 }
@@ -265,10 +441,7 @@ int launch(const ea_process_logits_t& a, cudaStream_t st) {
 template <typename T>
 int launch_type(const ea_process_logits_t& a, cudaStream_t st) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  // 16-byte pieces where input and output rows are equally far from a 16-byte boundary
-  const bool same = ((uintptr_t)a.logits - (uintptr_t)a.out) % 16 == 0 &&
-                    (a.rows <= 1 || (a.logits_stride - a.out_stride) % VEC == 0);
-  return same ? launch<T, VEC>(a, st) : launch<T, 1>(a, st);
+  return vec_of(a) == VEC ? launch<T, VEC>(a, st) : launch<T, 1>(a, st);
 }
 
 }  // namespace

@@ -4,7 +4,7 @@
 // A call through ctypes costs 20-25 us of interpreter time, several times what the small calls take on the
 // GPU; this module's calls cost 3-6 us. serving.py holds the documented functions, which pass their
 // arguments on by position. Wrong arguments raise ValueError, tensors off the GPU and CUDA errors RuntimeError.
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -89,6 +89,19 @@ void on_gpu(const at::Device& dev, const char* what) {
   if (!dev.is_cuda()) throw std::runtime_error(std::string(what) + " needs CUDA tensors (there is no CPU path)");
 }
 
+// An uninitialised tensor, without the dispatcher's share of at::empty.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
+  return at::detail::empty_cuda(sizes, type, dev, std::nullopt);
+}
+
+// `len` elements of a contiguous tensor from `off` on, sharing its storage.
+at::Tensor part(const at::Tensor& t, int64_t off, int64_t len) {
+  at::Tensor v = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+  v.unsafeGetTensorImpl()->set_storage_offset(t.storage_offset() + off);
+  v.unsafeGetTensorImpl()->set_sizes_contiguous(len);
+  return v;
+}
+
 template <typename F>
 PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F body) {
   if (n != want) {
@@ -145,9 +158,8 @@ PyObject* plan_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     need(batch <= EA_PLAN_MAX_SEQS, "plan_step: more than EA_PLAN_MAX_SEQS sequences");
     on_gpu(dev, "plan_step");
     c10::cuda::OptionalCUDAGuard guard(dev);
-    const auto opt = ctx.options();
-    at::Tensor slots = at::empty({cap}, opt.dtype(at::kLong));
-    at::Tensor per_tok = at::empty({2, cap}, opt), per_seq = at::empty({2 * batch + 3}, opt);
+    at::Tensor slots = fresh({cap}, at::kLong, dev);
+    at::Tensor per_tok = fresh({2 * cap}, at::kInt, dev), per_seq = fresh({2 * batch + 3}, at::kInt, dev);
     a.slot_map = slots.data_ptr<int64_t>();
     a.positions = per_tok.data_ptr<int32_t>(), a.token_seq = a.positions + cap;
     a.q_start = per_seq.data_ptr<int32_t>(), a.seq_lens = a.q_start + batch + 1;
@@ -156,9 +168,8 @@ PyObject* plan_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     a.batch = (int)batch, a.max_pages = (int)tab.size(1), a.page_size = (int)ps;
     a.num_free = (int)free_pages.size(0), a.max_tokens = (int)cap;
     call(ea_plan_step_cuda, a, dev);
-    const auto part = [&](int64_t off, int64_t len) { return per_seq.as_strided({len}, {1}, off); };
-    return tuple_of({slots, per_tok.as_strided({cap}, {1}, 0), per_tok.as_strided({cap}, {1}, cap), part(0, batch + 1),
-                     part(batch + 1, batch), part(2 * batch + 1, 1), part(2 * batch + 2, 1)});
+    return tuple_of({slots, part(per_tok, 0, cap), part(per_tok, cap, cap), part(per_seq, 0, batch + 1),
+                     part(per_seq, batch + 1, batch), part(per_seq, 2 * batch + 1, 1), part(per_seq, 2 * batch + 2, 1)});
   });
 }
 
@@ -222,9 +233,8 @@ PyObject* rope(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     on_gpu(dev, "rope");
     c10::cuda::OptionalCUDAGuard guard(dev);
     at::Tensor q_out, k_out;
-    const auto opt = first.options();
-    if (hq) q_out = at::empty({n, a.q_heads, d}, opt), a.q_out = q_out.data_ptr();
-    if (hk && !append) k_out = at::empty({n, a.kv_heads, d}, opt), a.k_out = k_out.data_ptr();
+    if (hq) q_out = fresh({n, a.q_heads, d}, type, dev), a.q_out = q_out.data_ptr();
+    if (hk && !append) k_out = fresh({n, a.kv_heads, d}, type, dev), a.k_out = k_out.data_ptr();
     call(ea_rope_cuda, a, dev);
     return tuple_of({q_out, k_out});
   });
@@ -267,9 +277,8 @@ PyObject* tree_attention(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     }
     on_gpu(dev, "tree_attention");
     c10::cuda::OptionalCUDAGuard guard(dev);
-    const auto opt = q.options();
-    if (!out.defined()) out = at::empty({n, hq, d}, opt);
-    if (v[9] == Py_True) lse = at::empty({n, hq}, opt.dtype(at::kFloat)), a.lse = lse.data_ptr<float>();
+    if (!out.defined()) out = fresh({n, hq, d}, type, dev);
+    if (v[9] == Py_True) lse = fresh({n, hq}, at::kFloat, dev), a.lse = lse.data_ptr<float>();
     a.q = q.data_ptr(), a.q_stride = q.stride(0), a.q_head_stride = q.stride(1);
     a.k_cache = kc.data_ptr(), a.k_page_stride = kc.stride(0), a.k_head_stride = kc.stride(1), a.k_row_stride = kc.stride(2);
     a.v_cache = vc.data_ptr(), a.v_page_stride = vc.stride(0), a.v_head_stride = vc.stride(1), a.v_row_stride = vc.stride(2);
@@ -282,7 +291,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     if (n && batch) {
       const int64_t bytes = ea_tree_attention_workspace(&a);
       if (bytes < 0) throw Refused(ea_serving_last_error());
-      ws = at::empty({bytes}, opt.dtype(at::kByte));
+      ws = fresh({bytes}, at::kByte, dev);
       a.workspace = ws.data_ptr();
     }
     call(ea_tree_attention_cuda, a, dev);
@@ -357,7 +366,7 @@ PyObject* process_logits(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     }
     on_gpu(dev, "process_logits");
     c10::cuda::OptionalCUDAGuard guard(dev);
-    if (!out.defined()) out = at::empty({rows, vocab}, x.options());
+    if (!out.defined()) out = fresh({rows, vocab}, x.scalar_type(), dev);
     a.logits = x.data_ptr(), a.logits_stride = x.stride(0), a.out = out.data_ptr(), a.out_stride = out.stride(0);
     a.rows = rows, a.vocab = (int)vocab, a.batch = (int)batch, a.dtype = type_code(x.scalar_type());
     call(ea_process_logits_cuda, a, dev);
