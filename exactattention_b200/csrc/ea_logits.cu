@@ -132,7 +132,7 @@ __device__ __forceinline__ float adjust(float x, uint32_t w, uint32_t token, con
 template <typename T, int VEC>
 __global__ void __launch_bounds__(DENSE_THREADS) dense_kernel(ea_process_logits_t a, int chunks, FastDiv by_chunks) {
   using P = Pack<T, VEC>;
-  cudaTriggerProgrammaticLaunchCompletion();
+  begin();
   const int64_t row = div_by(blockIdx.x, by_chunks);
   const int part = (int)(blockIdx.x - row * chunks);
   const T* src = (const T*)a.logits + row * a.logits_stride;
@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(DENSE_THREADS) dense_kernel(ea_process_logits_
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t a, int slots, int shift) {
+__global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t a, int slots, int shift, bool alone) {
+  if (alone) begin();
   extern __shared__ uint32_t keys[];  // token + 1, 0: free; then the words, then the list of used entries
   uint32_t* words = keys + slots;
   uint16_t* list = (uint16_t*)(words + slots);
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t 
   T* dst = (T*)a.out + row * a.out_stride;
   const uint32_t vocab = (uint32_t)a.vocab;
   if (n + n_bias == 0) {
-    cudaGridDependencySynchronize();  // nothing after this kernel may overtake the dense one
+    begin();  // nothing after this kernel may overtake the dense one
     return;
   }
   // One pass where the lists fit; else as many as the vocabulary needs, pass p taking the tokens that are p modulo
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t 
           ok |= (bits ? (bits[t >> 5] >> (t & 31)) & 1u : 1u) << e;
         }
       }
-      if (pass == 0 && first == 0) cudaGridDependencySynchronize();  // the dense kernel's rows are written
+      if (pass == 0 && first == 0) begin();  // the dense kernel's rows are written
 #pragma unroll
       for (int e = 0; e < BATCH; ++e) {
         if (!((ok >> e) & 1)) continue;
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t 
         dst[t] = from_f<T>(adjust(to_f(old[e]), words[tok[e]], t, r, ids, vals, n_bias, dup != 0));
       }
     }
-    if (pass == 0 && used == 0) cudaGridDependencySynchronize();
+    if (pass == 0 && used == 0) begin();
     __syncthreads();
   }
 }
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(THREADS, 2) chunk_kernel(ea_process_logits_t a, int chunk, int chunks, FastDiv by_chunks) {
   using P = Pack<T, VEC>;
+  begin();
   extern __shared__ uint4 table4[];
   uint32_t* table = (uint32_t*)table4;
   __shared__ uint16_t list[LIST];
@@ -409,15 +411,15 @@ int launch(const ea_process_logits_t& a, cudaStream_t st) {
   if (sparse && a.rows * chunks <= 4 * sm_count()) {
     chunk = (int)(((places + chunks - 1) / chunks + 15) & ~15ll);
     if ((e = allow_smem<chunk_kernel<T, VEC>>(4 * MAX_CHUNK)) != cudaSuccess) return cuda_rc(e);
-    chunk_kernel<T, VEC><<<(unsigned)(a.rows * chunks), THREADS, 4 * (size_t)chunk, st>>>(a, chunk, (int)chunks, fast_div((uint32_t)chunks));
-    return cuda_rc(cudaGetLastError());
+    return cuda_rc(launch_early(chunk_kernel<T, VEC>, (unsigned)(a.rows * chunks), THREADS, 4 * (size_t)chunk, st, a, chunk,
+                                (int)chunks, fast_div((uint32_t)chunks)));
   }
   if (dense) {
     const int per_block = UNROLL * DENSE_THREADS * VEC;
     chunks = (places + per_block - 1) / per_block;
     if (a.rows * chunks >= (1ll << 31)) return fail(-1, "process_logits: too many rows");
-    dense_kernel<T, VEC><<<(unsigned)(a.rows * chunks), DENSE_THREADS, 0, st>>>(a, (int)chunks, fast_div((uint32_t)chunks));
-    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_rc(e);
+    e = launch_early(dense_kernel<T, VEC>, (unsigned)(a.rows * chunks), DENSE_THREADS, 0, st, a, (int)chunks, fast_div((uint32_t)chunks));
+    if (e != cudaSuccess) return cuda_rc(e);
   }
   if (!sparse) return 0;
   if (a.rows >= (1ll << 31)) return fail(-1, "process_logits: too many rows");
@@ -426,16 +428,8 @@ int launch(const ea_process_logits_t& a, cudaStream_t st) {
   int log2 = 10;
   while ((1 << log2) < MAX_SLOTS && (1 << log2) / 4 * 3 < longest) ++log2;
   if ((e = allow_smem<sparse_kernel<T>>(MAX_SLOTS * 10)) != cudaSuccess) return cuda_rc(e);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.rows), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = (size_t)10 << log2;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr, cfg.numAttrs = dense ? 1 : 0;  // after the dense kernel only
-  e = cudaLaunchKernelEx(&cfg, sparse_kernel<T>, a, 1 << log2, 32 - log2);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return cuda_rc(e);
+  // alone (in place, without masks) it has to wait for what is before it; behind the dense kernel that one has
+  return cuda_rc(launch_early(sparse_kernel<T>, (unsigned)a.rows, THREADS, (size_t)10 << log2, st, a, 1 << log2, 32 - log2, !dense));
 }
 
 template <typename T>

@@ -56,6 +56,7 @@ __device__ __forceinline__ int pages_of(int64_t n, int ps) { return (int)((n + p
 __device__ __forceinline__ int32_t saturate(int64_t x) { return (int32_t)(x < 0x7FFFFFFF ? x : 0x7FFFFFFF); }
 
 __global__ void __launch_bounds__(THREADS) plan_step_kernel(ea_plan_step_t a, FastDiv by_page, bool vec) {
+  begin();
   extern __shared__ int32_t sm[];
   int32_t* tok = sm;                  // (batch + 1) prefix sums of the new tokens
   int32_t* frs = sm + a.batch + 1;    // (batch + 1) prefix sums of the fresh pages
@@ -186,6 +187,5 @@ extern "C" int ea_plan_step_cuda(const ea_plan_step_t* a, void* stream) {
   const int per_block = THREADS * PER_THREAD;
   const int grid = a->max_tokens > per_block ? (int)(((int64_t)a->max_tokens + per_block - 1) / per_block) : 1;
   const bool vec = (((uintptr_t)a->slot_map | (uintptr_t)a->positions | (uintptr_t)a->token_seq) & 15) == 0;
-  plan_step_kernel<<<grid, THREADS, smem, (cudaStream_t)stream>>>(*a, fast_div((uint32_t)a->page_size), vec);
-  return cuda_rc(cudaGetLastError());
+  return cuda_rc(launch_early(plan_step_kernel, grid, THREADS, smem, (cudaStream_t)stream, *a, fast_div((uint32_t)a->page_size), vec));
 }

@@ -61,6 +61,7 @@ __device__ __forceinline__ float2 cos_sin(int pos, float freq, bool inverse) {
 template <typename T, int VEC, int ITEMS, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : ITEMS == 4 ? 3 : 5) rope_kernel(ea_rope_t a, Plan p) {
   using P = Pack<T, VEC>;
+  begin();
   extern __shared__ float2 cs[];  // (tokens, rot / 2)
   const uint32_t group = div_by(blockIdx.x, p.by_head_blocks);
   const int64_t tok0 = (int64_t)group * p.tokens;
@@ -164,8 +165,7 @@ int launch_items(const ea_rope_t& a, Plan p, cudaStream_t st) {
   const int64_t blocks = (a.tokens + p.tokens - 1) / p.tokens * p.head_blocks;
   if (blocks >= (1ll << 31)) return fail(-1, "rope: too many tokens");
   // at most THREADS / units tokens of rot / 2 <= units * VEC pairs: 8 KB per VEC
-  rope_kernel<T, VEC, ITEMS, THREADS><<<(unsigned)blocks, THREADS, sizeof(float2) * p.tokens * (a.rot / 2), st>>>(a, p);
-  return cuda_rc(cudaGetLastError());
+  return cuda_rc(launch_early(rope_kernel<T, VEC, ITEMS, THREADS>, (unsigned)blocks, THREADS, sizeof(float2) * p.tokens * (a.rot / 2), st, a, p));
 }
 
 template <typename T, int VEC>

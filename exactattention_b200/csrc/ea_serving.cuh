@@ -30,6 +30,26 @@ __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_
 template <>
 __device__ __forceinline__ float from_f<float>(float x) { return x; }
 
+// Launches a kernel that may start while the one before it on the stream still runs (programmatic dependent launch), which
+// hides the launch's latency. Every block of every kernel here first calls begin(), which waits for all earlier work; only
+// the second kernel of a call may read the call's inputs before it.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e == cudaSuccess ? cudaGetLastError() : e;
+}
+// Waits for all earlier work on the stream, then lets the next kernel start.
+__device__ __forceinline__ void begin() {
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+}
+
 // n / d for n < 2^31 by one multiply: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
 // n / d = (umulhi(n, m) + n) >> s (the sum stays below 2^32 for n < 2^31).
 struct FastDiv {

@@ -145,7 +145,7 @@ __device__ __forceinline__ bool sees(const Args& a, const Item& it, int i, int k
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
   using S = Smem<DP>;
-  cudaTriggerProgrammaticLaunchCompletion();
+  begin();
   extern __shared__ uint8_t raw[];
   uint8_t* pool = (uint8_t*)(((uintptr_t)raw + 255) & ~(uintptr_t)255);
   uint32_t* sums = (uint32_t*)(raw + S::POOL);
@@ -425,8 +425,7 @@ int launch(Args& a, cudaStream_t st) {
     if (e == cudaSuccess && dev < 64) ready[dev] = true;
   }
   if (e != cudaSuccess) return cuda_rc(e);
-  few_rows_kernel<T, DP><<<a.workers, THREADS, smem, st>>>(a);
-  e = cudaGetLastError();
+  e = launch_early(few_rows_kernel<T, DP>, a.workers, THREADS, smem, st, a);
   if (e != cudaSuccess) return cuda_rc(e);
   return launch_combine<T, ROWS, KT>(a, st);
 }

@@ -114,16 +114,17 @@ constexpr int MANY_MAX_SEQS = 6000;  // what its shared memory has room for
 int launch_many(const Args& a, bool pair, cudaStream_t st);
 
 // Adds up the partials of the item that share blockIdx.x left unfinished, 16 rows a block (blockIdx.y). It starts
-// while the attention kernel still runs (programmatic dependent launch) and finds its item meanwhile.
-// Thread (share group, row, four channels): the groups take every G-th share, with all of a row's weights
-// 2^(m - max) computed once; the groups' sums are joined in a fixed order.
-constexpr int COMBINE_THREADS = 256, COMBINE_SHARES = 64;  // shares whose weights are held at a time
+// while the attention kernel still runs and finds its item meanwhile; after that its cost is the latency of two loads from
+// L2: all of a round's maxima, sums and values are asked for together.
+// Thread (share group, four channels, row): the groups take every G-th share; the groups' sums are joined in a fixed
+// order. A round is COMBINE_SHARES shares; between rounds what has been added up is rescaled to the new maximum.
+constexpr int COMBINE_THREADS = 256, COMBINE_SHARES = 16, COMBINE_AHEAD = 4;  // values a thread has in flight
 
 template <typename T, int ROWS, int KT>
 __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(Args a) {
   extern __shared__ uint32_t sums[];
   __shared__ uint64_t scratch[32];
-  __shared__ float weight[COMBINE_SHARES][16], top[16], total[16];
+  __shared__ float weight[COMBINE_SHARES][16], rescale[16], top[16], total[16];
   __shared__ float4 joined[COMBINE_THREADS];
   Schedule<ROWS, KT> sch;
   sch.build(a, sums, scratch);
@@ -133,74 +134,79 @@ __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(Args a) {
   int rows = 0, n = 2;  // rows of this block, shares of the item
   if (lo < hi) {
     it = sch.item(a, hi - 1, hi);
-    const uint32_t begin = hi - 1 - it.kt0, end = begin + it.tiles;  // the item's units
-    if (begin >= lo && end > hi) {                                   // begun here and not finished here
+    const uint32_t begin_unit = hi - 1 - it.kt0, end_unit = begin_unit + it.tiles;  // the item's units
+    if (begin_unit >= lo && end_unit > hi) {                                        // begun here and not finished here
       rows = min(16, min(ROWS, it.new_tokens * a.group - it.m * ROWS) - r0);
-      while (sch.share(w + n) < end) ++n;
+      while (sch.share(w + n) < end_unit) ++n;
     }
   }
-  cudaGridDependencySynchronize();
+  if (tid < 16) top[tid] = -INFINITY, total[tid] = 0.0f;
+  begin();
   if (rows <= 0) return;
   // partial i of the item: slot 2 w + 1, then slots 2 (w + i)
   const auto part = [&](int i) { return slot_of(a, i ? 2 * (w + i) : 2 * w + 1, ROWS); };
-
-  // maxima of the rows: 16 lanes a row
-  {
-    const int r = tid >> 4;
-    float m = -INFINITY;
-    if (r < rows)
-      for (int i = tid & 15; i < n; i += 16) m = fmaxf(m, part(i)[ROWS * a.dp + r0 + r]);
-#pragma unroll
-    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((tid & 15) == 0) top[r] = m, total[r] = 0.0f;
-  }
   const int vecs = a.dp / 4, cells = rows * vecs;  // at most 512: two cells a thread where there are many rows
-  int groups = COMBINE_THREADS / cells;            // groups of threads that take every groups-th share
-  if (groups < 1) groups = 1;
+  const int groups = max(1, COMBINE_THREADS / cells);
   const int grp = min(tid / cells, groups), cell0 = cells > COMBINE_THREADS ? tid : tid - tid / cells * cells;
+  const int mr = tid >> 4, ms = tid & 15;  // the row and share whose maximum and sum this thread reads
   float4 acc[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
   for (int i0 = 0; i0 < n; i0 += COMBINE_SHARES) {
     const int m = min(COMBINE_SHARES, n - i0);
-    __syncthreads();
-    {
-      const int r = tid >> 4;
-      float l = 0.0f;
-      if (r < rows) {
-        const float base = top[r] == -INFINITY ? 0.0f : top[r];
-        for (int i = tid & 15; i < m; i += 16) {
-          const float* p = part(i0 + i) + ROWS * a.dp + r0 + r;
-          const float f = exp2f(p[0] - base);
-          weight[i][r] = f;
-          l = fmaf(p[ROWS], f, l);
-        }
-      }
-#pragma unroll
-      for (int o = 8; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      if ((tid & 15) == 0) total[r] += l;
+    float pm = -INFINITY, pl = 0.0f;
+    if (mr < rows && ms < m) {
+      const float* p = part(i0 + ms) + ROWS * a.dp + r0 + mr;
+      pm = p[0], pl = p[ROWS];
     }
-    __syncthreads();
-    if (grp < groups)
+    float4 x[2][COMBINE_AHEAD];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int cell = cell0 + c * COMBINE_THREADS;
-        if (cell >= cells) break;
-        const int v = cell / rows, r = cell - v * rows, at = (v * ROWS + r0 + r) * 4;
-#pragma unroll 4
-        for (int i = grp; i < m; i += groups) {
-          const float4 x = *(const float4*)(part(i0 + i) + at);
-          const float f = weight[i][r];
-          acc[c].x = fmaf(x.x, f, acc[c].x), acc[c].y = fmaf(x.y, f, acc[c].y);
-          acc[c].z = fmaf(x.z, f, acc[c].z), acc[c].w = fmaf(x.w, f, acc[c].w);
+    for (int c = 0; c < 2; ++c) {
+      const int cell = cell0 + c * COMBINE_THREADS, v = cell / rows, at = (v * ROWS + r0 + cell - v * rows) * 4;
+#pragma unroll
+      for (int j = 0; j < COMBINE_AHEAD; ++j)
+        if (grp < groups && cell < cells && grp + j * groups < m) x[c][j] = *(const float4*)(part(i0 + grp + j * groups) + at);
+    }
+    float best = pm;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    __syncthreads();  // the last round's weights are used (and top is set)
+    const float was = top[mr], now = fmaxf(was, best), base = now == -INFINITY ? 0.0f : now;
+    const float f = exp2f(pm - base), old = exp2f(was - base);
+    float l = pl * f;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    weight[ms][mr] = f;
+    __syncwarp();  // top and total are read by the row's lanes, which are in one warp
+    if (ms == 0) top[mr] = now, total[mr] = fmaf(total[mr], old, l), rescale[mr] = old;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int cell = cell0 + c * COMBINE_THREADS;
+      if (grp >= groups || cell >= cells) continue;
+      const int v = cell / rows, r = cell - v * rows, at = (v * ROWS + r0 + r) * 4;
+      if (i0) acc[c].x *= rescale[r], acc[c].y *= rescale[r], acc[c].z *= rescale[r], acc[c].w *= rescale[r];
+      int j = 0;
+      for (int i = grp; i < m; i += groups, ++j) {
+        float4 y;
+        if (j < COMBINE_AHEAD) {
+#pragma unroll
+          for (int k = 0; k < COMBINE_AHEAD; ++k)
+            if (k == j) y = x[c][k];
+        } else {
+          y = *(const float4*)(part(i0 + i) + at);
         }
+        const float g = weight[i][r];
+        acc[c].x = fmaf(y.x, g, acc[c].x), acc[c].y = fmaf(y.y, g, acc[c].y);
+        acc[c].z = fmaf(y.z, g, acc[c].z), acc[c].w = fmaf(y.w, g, acc[c].w);
       }
+    }
   }
   if (groups > 1) {
     joined[tid] = acc[0];
     __syncthreads();
     if (tid < cells)
       for (int g = 1; g < groups; ++g) {
-        const float4 x = joined[g * cells + tid];
-        acc[0].x += x.x, acc[0].y += x.y, acc[0].z += x.z, acc[0].w += x.w;
+        const float4 y = joined[g * cells + tid];
+        acc[0].x += y.x, acc[0].y += y.y, acc[0].z += y.z, acc[0].w += y.w;
       }
   }
   if (grp > 0) return;
@@ -224,16 +230,8 @@ __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(Args a) {
 template <typename T, int ROWS, int KT>
 int launch_combine(const Args& a, cudaStream_t st) {
   if (a.workers <= 1) return 0;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.workers, ROWS / 16), cfg.blockDim = dim3(COMBINE_THREADS);
-  cfg.dynamicSmemBytes = 4 * (size_t)(a.t.batch + 1), cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, combine_kernel<T, ROWS, KT>, a);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return cuda_rc(e);
+  return cuda_rc(launch_early(combine_kernel<T, ROWS, KT>, dim3((unsigned)a.workers, ROWS / 16), COMBINE_THREADS,
+                              4 * (size_t)(a.t.batch + 1), st, a));
 }
 
 }  // namespace tree

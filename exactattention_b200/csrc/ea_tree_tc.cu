@@ -69,8 +69,7 @@ int launch(const Args& a, cudaStream_t st) {
   CUtensorMap tk, tv;
   int box = box_rows(a.t.page_size);
   if (box && !(tensor_map(a, false, box, &tk) && tensor_map(a, true, box, &tv))) box = 0;
-  many::many_rows_kernel<T, DP, PAIR><<<a.workers, many::THREADS, C::SMEM + sums, st>>>(a, tk, tv, box);
-  e = cudaGetLastError();
+  e = launch_early(many::many_rows_kernel<T, DP, PAIR>, a.workers, many::THREADS, C::SMEM + sums, st, a, tk, tv, box);
   if (e != cudaSuccess) return cuda_rc(e);
   return launch_combine<T, C::ROWS, many::KT>(a, st);
 }

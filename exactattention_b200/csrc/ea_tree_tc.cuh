@@ -280,7 +280,6 @@ __device__ __noinline__ void add_not_finite(const Args& a, const Item& it, int i
 template <typename T, int DP, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     many_rows_kernel(Args a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, int box) {
-  cudaTriggerProgrammaticLaunchCompletion();
   using C = Cfg<DP, PAIR>;
   constexpr int ROWS = C::ROWS, NBUF = C::NBUF, BUF = C::BUF;
   extern __shared__ uint8_t raw[];
@@ -291,8 +290,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint32_t* sums = (uint32_t*)(raw + C::SMEM);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  Schedule<ROWS, KT> sch;
-  sch.build(a, sums, sh.scratch);
   if (tid == 0) {
     for (int i = 0; i < NBUF; ++i) mbar_init(&sh.full[i], box ? 1 : LOADERS), mbar_init(&sh.empty[i], 1);
     for (int s = 0; s < 2; ++s) mbar_init(&sh.s_full[s], 1), mbar_init(&sh.p_ready[s], SLOT_THREADS);
@@ -301,6 +298,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     sh.dirty[0][0] = sh.dirty[0][1] = sh.dirty[1][0] = sh.dirty[1][1] = 0;
   }
   if (warp == 8) tmem_alloc(&sh.tmem, 512);
+  begin();
+  Schedule<ROWS, KT> sch;
+  sch.build(a, sums, sh.scratch);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
