@@ -25,7 +25,8 @@ struct Item {
   int b, h, m;            // sequence, kv head, row tile
   int q0, new_tokens;     // first token of the step and their number
   int len;                // keys, the step's own included
-  int kt0, kt1, tiles;    // key tiles of this share, and of the item
+  int kt0, kt1, tiles;    // key tiles of this share (none: kt0 >= kt1), and of the item
+  uint32_t next;          // unit after the share's part of the item
 };
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
@@ -36,7 +37,7 @@ __device__ __forceinline__ void seq_tokens(const Args& a, int b, int& q0, int& n
   q0 = (int)lo, n = (int)max(hi - lo, (int64_t)0);
 }
 
-template <int ROWS, int KT>
+template <int ROWS, int KT, int EXTRA>
 struct Schedule {
   const uint32_t* prefix;  // (batch + 1) in shared memory
   uint32_t total, workers;  // units; blocks that get some (a block past them has nothing to do)
@@ -52,7 +53,7 @@ struct Schedule {
         int q0, nt;
         seq_tokens(a, b, q0, nt);
         u = (uint64_t)a.t.kv_heads * (uint32_t)((nt * a.group + ROWS - 1) / ROWS) *
-            (uint32_t)max(1, (seq_len(a, b) + KT - 1) / KT);
+            (uint32_t)(max(1, (seq_len(a, b) + KT - 1) / KT) + EXTRA);
       }
       uint64_t s = u;
 #pragma unroll
@@ -94,9 +95,10 @@ struct Schedule {
     it.len = seq_len(a, lo);
     it.tiles = max(1, (it.len + KT - 1) / KT);
     const uint32_t mt = (uint32_t)((it.new_tokens * a.group + ROWS - 1) / ROWS);
-    const uint32_t rel = pos - prefix[lo], idx = rel / (uint32_t)it.tiles;
-    it.kt0 = (int)(rel - idx * it.tiles);
-    it.kt1 = (int)min((uint32_t)it.tiles, it.kt0 + (end - pos));
+    const uint32_t units = it.tiles + EXTRA, rel = pos - prefix[lo], idx = rel / units, at = rel - idx * units;
+    it.kt0 = (int)at;
+    it.kt1 = (int)min((uint32_t)it.tiles, at + (end - pos));
+    it.next = pos + min(end - pos, units - at);
     it.h = (int)(idx / mt), it.m = (int)(idx - it.h * mt);
     return it;
   }
@@ -120,13 +122,13 @@ int launch_many(const Args& a, bool pair, cudaStream_t st);
 // order. A round is COMBINE_SHARES shares; between rounds what has been added up is rescaled to the new maximum.
 constexpr int COMBINE_THREADS = 256, COMBINE_SHARES = 16, COMBINE_AHEAD = 4;  // values a thread has in flight
 
-template <typename T, int ROWS, int KT>
+template <typename T, int ROWS, int KT, int EXTRA>
 __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(Args a) {
   extern __shared__ uint32_t sums[];
   __shared__ uint64_t scratch[32];
   __shared__ float weight[COMBINE_SHARES][16], rescale[16], top[16], total[16];
   __shared__ float4 joined[COMBINE_THREADS];
-  Schedule<ROWS, KT> sch;
+  Schedule<ROWS, KT, EXTRA> sch;
   sch.build(a, sums, scratch);
   const int w = blockIdx.x, tid = threadIdx.x, r0 = blockIdx.y * 16;
   const uint32_t lo = sch.share(w), hi = sch.share(w + 1);
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(Args a) {
   if (lo < hi) {
     it = sch.item(a, hi - 1, hi);
     const uint32_t begin_unit = hi - 1 - it.kt0, end_unit = begin_unit + it.tiles;  // the item's units
-    if (begin_unit >= lo && end_unit > hi) {                                        // begun here and not finished here
+    if (begin_unit >= lo && end_unit > hi) {  // begun here and not finished here
       rows = min(16, min(ROWS, it.new_tokens * a.group - it.m * ROWS) - r0);
       while (sch.share(w + n) < end_unit) ++n;
     }
@@ -227,10 +229,10 @@ __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(Args a) {
 }
 
 // Launches the combine kernel right after an attention kernel on the stream.
-template <typename T, int ROWS, int KT>
+template <typename T, int ROWS, int KT, int EXTRA>
 int launch_combine(const Args& a, cudaStream_t st) {
   if (a.workers <= 1) return 0;
-  return cuda_rc(launch_early(combine_kernel<T, ROWS, KT>, dim3((unsigned)a.workers, ROWS / 16), COMBINE_THREADS,
+  return cuda_rc(launch_early(combine_kernel<T, ROWS, KT, EXTRA>, dim3((unsigned)a.workers, ROWS / 16), COMBINE_THREADS,
                               4 * (size_t)(a.t.batch + 1), st, a));
 }
 

@@ -71,7 +71,7 @@ int launch(const Args& a, cudaStream_t st) {
   if (box && !(tensor_map(a, false, box, &tk) && tensor_map(a, true, box, &tv))) box = 0;
   e = launch_early(many::many_rows_kernel<T, DP, PAIR>, a.workers, many::THREADS, C::SMEM + sums, st, a, tk, tv, box);
   if (e != cudaSuccess) return cuda_rc(e);
-  return launch_combine<T, C::ROWS, many::KT>(a, st);
+  return launch_combine<T, C::ROWS, many::KT, many::EXTRA>(a, st);
 }
 
 }  // namespace

@@ -18,6 +18,11 @@
 // share the reference).
 // Weights are rounded to the cache's type for the product (relative error 2^-9 for bf16, 2^-12 for fp16, of
 // random sign, about the rounding of the output itself); their sum takes them unrounded.
+// Measured on one B200: 16 trees of 17 to 64 nodes over 1K to 15K keys, 16 / 8 heads of 128, 144 us (545 MB of keys and
+// values: 83 us at the copy rate); four chunks of 256 tokens behind 16K keys, 32 / 4 heads, 333 us (277 GFLOP: 170 us at
+// the measured bf16 rate; the tensor pipe is active 42% of the time). A slot's cycle at 128 x 128 x 128 is what bounds it:
+// some 1900 cycles for the weights, 400 to store them and hand them over, 1750 for the issue of the 16 products beside
+// busy softmax warps, 400 until the scores are seen, 4800 in all for both slots' tiles.
 #pragma once
 #include <cuda.h>
 
@@ -37,6 +42,7 @@ constexpr int SLOT_THREADS = 128, LOADERS = 64;
 constexpr int LAUNCH_REGS = 168, SLOT_REGS = 216, OTHER_REGS = 72;
 constexpr uint32_t COL_S = 0, COL_O = 256;  // slot s: + 128 s
 constexpr int PAGE_RING = 16;
+constexpr int EXTRA = 3;  // units for an item's end: some 8000 cycles against 2400 to 2800 of a tile
 
 template <int DP, bool PAIR>
 struct Cfg {
@@ -299,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   if (warp == 8) tmem_alloc(&sh.tmem, 512);
   begin();
-  Schedule<ROWS, KT> sch;
+  Schedule<ROWS, KT, EXTRA> sch;
   sch.build(a, sums, sh.scratch);
   fence_before_sync();
   __syncthreads();
@@ -317,7 +323,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t items = 0;
     while (pos < end && alive) {
       const Item it = sch.item(a, pos, end);
-      pos += it.kt1 - it.kt0;
+      pos = it.next;
+      if (it.kt0 >= it.kt1) continue;
       if (items) alive = __all_sync(0xffffffffu, wait_phase(&sh.q_free, (items - 1) & 1));
       if (!alive) break;
       ++items;
@@ -351,7 +358,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t cnt = 0, tile0 = 0;  // tiles loaded; key tiles of earlier items
       while (pos < end && alive) {
         const Item it = sch.item(a, pos, end);
-        pos += it.kt1 - it.kt0;
+        pos = it.next;
+        if (it.kt0 >= it.kt1) continue;
         const int n = it.kt1 - it.kt0;
         const auto page_of = [&](int t) {
           const int key = (it.kt0 + t) * KT + sub * box;
@@ -422,7 +430,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     while (pos < end && alive) {
       const Item it = sch.item(a, pos, end);
-      pos += it.kt1 - it.kt0;
+      pos = it.next;
+      if (it.kt0 >= it.kt1) continue;
       const int n = it.kt1 - it.kt0;
       const auto page_of = [&](int t, int half) {
         const int key = (it.kt0 + t) * KT + w2 * 64 + half * 32 + lane;
@@ -492,7 +501,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       while (pos < end && alive) {
         const Item it = sch.item(a, pos, end);
-        pos += it.kt1 - it.kt0;
+        pos = it.next;
+        if (it.kt0 >= it.kt1) continue;
         const int n = it.kt1 - it.kt0;
         const int slots = !PAIR || it.new_tokens * a.group - it.m * ROWS > TILE ? 2 : 1;  // PAIR: slots with rows
         if (items) wait(&sh.seen, (items - 1) & 1);  // the slots have seen the end of the last item
@@ -561,7 +571,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     while (pos < end) {
       const Item it = sch.item(a, pos, end);
-      pos += it.kt1 - it.kt0;
+      pos = it.next;
+      if (it.kt0 >= it.kt1) continue;
       const int n = it.kt1 - it.kt0, ctx = it.len - it.new_tokens;
       const int all_rows = it.new_tokens * a.group - it.m * ROWS;
       const int rows = min(TILE, all_rows - (PAIR ? slot * TILE : 0));  // of this slot's tile; may be <= 0 for PAIR
@@ -583,7 +594,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int c = 0; c < KT / 32; ++c) vis[c] = seen_word(a, it, tok, key0 + c * 32) & ok[c];
           }
-          // One pass in the common case: the weights against the maximum so far, while the tile's own maximum is taken.
+          // One pass in the common case (a first pass for the maximum alone cost 500 cycles of a tile's 2650; holding the whole
+          // tile's scores in registers spilled): the weights against the maximum so far, while the tile's own is taken.
           // They are stored, over the scores, only if no row's maximum grew by more than 8; else O is rescaled and
           // a second pass computes them anew. A slot's first tile takes its maximum before.
           uint32_t u[2][16], p[KT / 2];

@@ -7,7 +7,8 @@ B200 library `exactattention_b200`, so that callers written against the referenc
     from exactattn.cuda import attention_cuda     # the CUDA counterpart of exactattn.cpu.attention_cpu
 
 `exactattn.cuda`, `exactattn.torch_impl` and `exactattn.formats` are the B200 package's modules
-under those names. The reference's `trace_row` (exact intermediates for debugging) is not
+under those names; the serving operators have no counterpart in the reference and are reached as
+`exactattention_b200.serving`. The reference's `trace_row` (exact intermediates for debugging) is not
 provided: it belongs to the reference's pure-Python ground truth, not to the attention path.
 """
 

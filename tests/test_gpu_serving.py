@@ -291,6 +291,28 @@ def test_tree_attention_infinite_values_in_the_context():
     check_attention(y)
 
 
+@pytest.mark.parametrize("alpha", [-0.2, 0.0, 1e-9])
+@pytest.mark.parametrize("new", [1, 30])
+def test_tree_attention_any_alpha(alpha, new):
+    x = attention_inputs([150, 0], [new, 3], 8, 2, 128, 16, torch.bfloat16)
+    check_attention(dict(x, alpha=alpha))
+
+
+def test_tree_attention_more_sequences_than_the_tensor_core_kernel_takes():
+    x = attention_inputs([3] * 6100, [1] * 6099 + [40], 2, 1, 64, 16, torch.bfloat16, mask="chain")
+    check_attention(x, max_new=40)
+
+
+def test_tree_attention_out_and_unused_rows():
+    x = attention_inputs([90, 20], [9, 40], 8, 2, 128, 16, torch.bfloat16)
+    want = serving.tree_attention(**x)
+    q = torch.cat([x["q"], x["q"][:7]])  # rows past the step's tokens, as a padded step has them
+    mask = torch.cat([x["tree_mask"], x["tree_mask"][:7]])
+    out = torch.full(q.shape, 5.0, dtype=q.dtype, device=DEV)
+    assert serving.tree_attention(**dict(x, q=q, tree_mask=mask), out=out) is out
+    assert torch.equal(out[:49], want) and bool((out[49:] == 5).all())
+
+
 def test_tree_attention_cache_past_32_bit_offsets():
     hk, ps, d = 2, 64, 128
     pages = 2**31 // (hk * ps * d) + 60
