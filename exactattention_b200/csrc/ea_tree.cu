@@ -1,18 +1,18 @@
 // Attention of a step's tokens over the paged cache (ea_tree_attention_cuda): the entry, and the kernel for
 // few query rows per kv head.
 //
-// Row statistics (maximum, sum) and outputs are binary32. The kernel below keeps 16 query rows of one
-// sequence and kv head (tokens x the heads of a group) in registers as the A operand of 16 x 8 x 16 matrix
-// instructions; a warp owns 16 of a tile's 64 keys with a running maximum, sum and output of its own, so the
-// warps of a block stream their keys without waiting for one another and join once per item. Bound by HBM:
-// a 16-key slice is 8 KB of K and V at d = 128, for which an SM has about 350 cycles at the
-// measured copy rate, and needs 48 matrix instructions and 16 ldmatrix of its four sub-partitions.
-// Weights enter P.V as a pair of 16-bit numbers, their rounding and its remainder (relative
-// error 2^-17 for bf16 instead of 2^-9), which costs 16 more matrix instructions a slice: the tensor pipe
-// has the room (27% active).
-// Measured on one B200: 64 sequences of 4K to 32K keys, 16 / 8 heads of 128, pages of 16 in random order: 780 to 870 us
-// from run to run for 4.83 GB (85 to 94% of the copy rate); one token over 777 keys: 9.3 us, most of it latency (start 1,
-// lengths to first copies 1.5, keys and products 2, join and partials 1, the combine kernel 3).
+// Row statistics (maximum, sum) and outputs are binary32. The kernel below keeps the query rows of one sequence and kv
+// head (tokens x the heads of a group, 8 or 16) in registers as the narrow operand of 16 x 8 x 16 matrix instructions:
+// keys are the M side of the scores, channels the M side of the outputs, rows the N side of both, so few rows
+// cost few instructions. With rows on the M side two rows cost what sixteen do: 64 sequences of 4096 to 32768 keys,
+// 2 rows, d = 128 took 776 us in bursts and 860 us in a long loop, where the 1000 W limit lowered the SM clock to 1.7 to
+// 1.85 GHz; this way round takes 737 us and 790 us. Sixteen rows lose to the turning over of the weights: 895 us before,
+// 915 us now in a long loop (d = 128). A warp owns 16 of a tile's 64 keys with a running maximum, sum and output of its
+// own, so the warps of a block stream their keys without waiting for one another and join once per item. Bound by HBM: a
+// 16-key slice is 8 KB of K and V at d = 128, for which an SM has about 350 cycles at the measured copy rate, and
+// needs 24 matrix instructions (8 rows; 48 for 16) and 16 ldmatrix of its four sub-partitions.
+// Weights enter P.V as a pair of 16-bit numbers, their rounding and its remainder (relative error 2^-17 for bf16
+// instead of 2^-9), which is 8 of those 24 instructions: the tensor pipe has the room.
 #include <type_traits>
 
 #include "ea_tree.cuh"
@@ -23,7 +23,11 @@ namespace tree {
 
 namespace {
 
-constexpr int ROWS = 16, WARPS = 4, KT = 16 * WARPS, THREADS = 32 * WARPS, STAGES = 3, EXTRA = 1;
+constexpr int MAX_ROWS = 16, WARPS = 4, KT = 16 * WARPS, THREADS = 32 * WARPS, STAGES = 3, EXTRA = 1;
+
+// A row's reference moves only when a score passes it by more than this (in powers of two): the weights are then at
+// most 256, which both types hold with the same relative error, and most slices need no reduction over lanes.
+constexpr float LAZY = 8.0f;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -48,11 +52,17 @@ __device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t* r) {
                : "r"(a)
                : "memory");
 }
+// an 8 x 8 matrix of 16-bit numbers, two of a row in each lane, turned over
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
       "%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -60,7 +70,7 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float* c, const uint32_t* a, 
 }
 template <>
 __device__ __forceinline__ void mma<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
       "%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -103,7 +113,7 @@ struct Smem {
   static constexpr int SLICE = 16 * ROW_BYTES;                    // K or V of 16 keys
   static constexpr int STAGE = 2 * SLICE;                         // one warp's
   static constexpr int POOL = WARPS * STAGES * STAGE + 256;       // aligned to 256 bytes; also the join's scratch
-  static_assert(POOL - 256 >= WARPS * ROWS * DP * 4, "the join fits into the stages");
+  static_assert(POOL - 256 >= WARPS * MAX_ROWS * DP * 4, "the join fits into the stages");
 };
 
 template <int DP>
@@ -145,9 +155,10 @@ __device__ __forceinline__ bool sees(const Args& a, const Item& it, int i, int k
   return (j >> 5) < a.t.mask_words && ((a.t.tree_mask[(int64_t)(it.q0 + i) * a.t.mask_words + (j >> 5)] >> (j & 31)) & 1);
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(Args a) {
   using S = Smem<DP>;
+  constexpr int ROWS = 8 * NT;
   begin();
   extern __shared__ uint8_t raw[];
   uint8_t* pool = (uint8_t*)(((uintptr_t)raw + 255) & ~(uintptr_t)255);
@@ -170,8 +181,8 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
   const int64_t k_lane = (lane / LPR) * a.t.k_row_stride + (bytes0 ? c0 * 8 : 0);
   const int64_t v_lane = (lane / LPR) * a.t.v_row_stride + (bytes0 ? c0 * 8 : 0);
   // fragment addresses inside a slice; a step of 16 channels flips address bits 5 and up
-  const uint32_t k_frag = ((lane & 7) + ((lane >> 4) << 3)) * S::ROW_BYTES + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
-  const uint32_t v_frag = S::SLICE + (lane & 15) * S::ROW_BYTES + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t k_frag = (lane & 15) * S::ROW_BYTES + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_frag = S::SLICE + ((lane & 7) + ((lane >> 4) << 3)) * S::ROW_BYTES + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 
   while (pos < end) {
     const Item it = sch.item(a, pos, end);
@@ -181,23 +192,23 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
     const int rows = min(ROWS, it.new_tokens * a.group - it.m * ROWS);
     const int R0 = it.m * ROWS;
 
-    // Q as A fragments: rows lane / 4 and lane / 4 + 8
-    uint32_t qf[DP / 16][4];
-    int tok[2];
+    // Q as B fragments: row 8 nt + lane / 4; and the tokens of the rows whose statistics this lane keeps, 8 nt +
+    // 2 (lane % 4) + e
+    uint32_t qf[NT][DP / 16][2];
+    int tok[NT][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = lane / 4 + 8 * half, R = R0 + min(r, rows - 1);
-      tok[half] = (int)div_by((uint32_t)R, a.by_group);
-      const int j = R - tok[half] * a.group;
-      const T* q = (const T*)a.t.q + (int64_t)(it.q0 + tok[half]) * a.t.q_stride +
-                   (int64_t)(it.h * a.group + j) * a.t.q_head_stride;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int R = R0 + min(8 * nt + lane / 4, rows - 1), i = (int)div_by((uint32_t)R, a.by_group);
+      const T* q = (const T*)a.t.q + (int64_t)(it.q0 + i) * a.t.q_stride + (int64_t)(it.h * a.group + R - i * a.group) * a.t.q_head_stride;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int c = ks * 16 + p * 8 + (lane & 3) * 2;
-          qf[ks][half + 2 * p] = c < a.t.d ? *(const uint32_t*)(q + c) : 0u;
+          qf[nt][ks][p] = c < a.t.d ? *(const uint32_t*)(q + c) : 0u;
         }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) tok[nt][e] = (int)div_by((uint32_t)(R0 + min(8 * nt + 2 * (lane & 3) + e, rows - 1)), a.by_group);
     }
     const int n = it.kt1 - it.kt0;
     const int key_w = it.kt0 * KT + warp * 16;
@@ -236,16 +247,20 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
       return __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
     };
 
-    float o[DP / 8][4], m[2], l[2];
+    // o: channels 16 nn + lane / 4 (+ 8), rows 8 nt + 2 (lane % 4) (+ 1)
+    float o[NT][DP / 16][4], m[NT][2], l[NT][2];
     // The first pass takes the values as they are. An infinity or NaN among them may not meet the zero weight of a row
     // that does not see its key, nor a weight's remainder: if any output is not finite, a second pass takes
     // such values out of the product and adds them to the rows that see them one by one.
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-      for (int nn = 0; nn < DP / 8; ++nn)
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[nn][e] = 0.0f;
-      m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.0f;
+        for (int nn = 0; nn < DP / 16; ++nn)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][nn][e] = 0.0f;
+        m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.0f;
+      }
       uint32_t exist[STAGES];  // of the slices under way, oldest first
       int page = page_of(key_w);
 #pragma unroll
@@ -258,69 +273,71 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
       for (int t = 0; t < n; ++t) {
         cp_wait<STAGES - 2>();
         __syncwarp();
-        const int nt = t + STAGES - 1;
-        exist[STAGES - 1] = nt < n ? load(key_w + nt * KT, page, ahead) : 0;
+        const int coming = t + STAGES - 1;
+        exist[STAGES - 1] = coming < n ? load(key_w + coming * KT, page, ahead) : 0;
         cp_commit();
-        page = page_of(key_w + (nt + 1) * KT);
+        page = page_of(key_w + (coming + 1) * KT);
         const int key0 = key_w + t * KT;
         const uint32_t okm = exist[0];
 
-        // scores: s[nt][..] rows lane / 4 (+ 8), keys nt * 8 + 2 (lane % 4) (+ 1)
-        float s[2][4];
+        // scores: keys lane / 4 (+ 8), rows 8 nt + 2 (lane % 4) (+ 1)
+        float s[NT][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.0f;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
           if (ks * 16 < a.t.d) {
             uint32_t f[4];
             ldsm4((cur + k_frag) ^ (ks * 32), f);
-            mma<T>(s[0], qf[ks], f[0], f[1]);
-            mma<T>(s[1], qf[ks], f[2], f[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma<T>(s[nt], f, qf[nt][ks][0], qf[nt][ks][1]);
           }
         }
+        const bool masked = key0 + 16 > ctx || okm != 0xFFFFu;
+        uint32_t hi[NT][2], lo[NT][2];
+        bool grows = false;
 #pragma unroll
-        for (int nt2 = 0; nt2 < 2; ++nt2)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt2][e] *= alpha;
-        if (key0 + 16 > ctx || okm != 0xFFFFu) {
-#pragma unroll
-          for (int nt2 = 0; nt2 < 2; ++nt2)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int kk = nt2 * 8 + 2 * (lane & 3) + (e & 1);
-              if (!sees(a, it, tok[e >> 1], key0 + kk, (okm >> kk) & 1)) s[nt2][e] = -INFINITY;
+          for (int e = 0; e < 4; ++e) {
+            s[nt][e] *= alpha;
+            if (masked) {
+              const int kk = (lane >> 2) + 8 * (e >> 1);
+              if (!sees(a, it, tok[nt][e & 1], key0 + kk, (okm >> kk) & 1)) s[nt][e] = -INFINITY;
             }
-        }
-        float scale[2];
+            grows |= s[nt][e] > m[nt][e & 1] + LAZY;
+          }
+        if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float mx = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float mn = fmaxf(m[half], mx), ref = mn == -INFINITY ? 0.0f : mn;
-          scale[half] = ex2(m[half] - ref);
-          m[half] = mn;
-          l[half] *= scale[half];
-#pragma unroll
-          for (int nt2 = 0; nt2 < 2; ++nt2)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              s[nt2][2 * half + e] = ex2(s[nt2][2 * half + e] - ref);
-              l[half] += s[nt2][2 * half + e];
+              float mx = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][2 + e]));
+#pragma unroll
+              for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+              const float scale = ex2(m[nt][e] - (mx == -INFINITY ? 0.0f : mx));
+              m[nt][e] = mx, l[nt][e] *= scale;
+#pragma unroll
+              for (int nn = 0; nn < DP / 16; ++nn) o[nt][nn][e] *= scale, o[nt][nn][2 + e] *= scale;
             }
         }
-        if (__any_sync(0xffffffffu, scale[0] != 1.0f || scale[1] != 1.0f)) {
 #pragma unroll
-          for (int nn = 0; nn < DP / 8; ++nn)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[nn][e] *= scale[e >> 1];
+          for (int e = 0; e < 2; ++e) {
+            const float ref = m[nt][e] == -INFINITY ? 0.0f : m[nt][e];
+            s[nt][e] = ex2(s[nt][e] - ref), s[nt][2 + e] = ex2(s[nt][2 + e] - ref);
+            l[nt][e] += s[nt][e] + s[nt][2 + e];
+          }
+          // the weights as B fragments: keys 2 (lane % 4) (+ 1) (+ 8), row lane / 4
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            split2<T>(s[nt][2 * h], s[nt][2 * h + 1], hi[nt][h], lo[nt][h]);
+            hi[nt][h] = transpose8(hi[nt][h]), lo[nt][h] = transpose8(lo[nt][h]);
+          }
         }
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int nt2 = 0; nt2 < 2; ++nt2)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            split2<T>(s[nt2][2 * half], s[nt2][2 * half + 1], hi[nt2 * 2 + half], lo[nt2 * 2 + half]);
 #pragma unroll
         for (int nn = 0; nn < DP / 16; ++nn) {
           if (nn * 16 < a.t.d) {
@@ -330,24 +347,31 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) f[e] = finite2<T>(f[e]);
             }
-            mma<T>(o[2 * nn], hi, f[0], f[1]);
-            mma<T>(o[2 * nn + 1], hi, f[2], f[3]);
-            mma<T>(o[2 * nn], lo, f[0], f[1]);
-            mma<T>(o[2 * nn + 1], lo, f[2], f[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma<T>(o[nt][nn], f, hi[nt][0], hi[nt][1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma<T>(o[nt][nn], f, lo[nt][0], lo[nt][1]);
           }
         }
         if (pass) {
           for (int kk = 0; kk < 16; ++kk) {
-            const bool see0 = sees(a, it, tok[0], key0 + kk, (okm >> kk) & 1), see1 = sees(a, it, tok[1], key0 + kk, (okm >> kk) & 1);
+            bool see[NT][2];
 #pragma unroll
-            for (int nn = 0; nn < DP / 8; ++nn)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int c = nn * 8 + 2 * (lane & 3) + e;
+              for (int e = 0; e < 2; ++e) see[nt][e] = sees(a, it, tok[nt][e], key0 + kk, (okm >> kk) & 1);
+#pragma unroll
+            for (int nn = 0; nn < DP / 16; ++nn)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int c = nn * 16 + 8 * h + (lane >> 2);
                 const float f = to_f(*(const T*)(pool + (cur - smem_addr(pool)) + S::SLICE + swz<DP>(kk, c >> 3) + (c & 7) * 2));
                 if (isfinite(f)) continue;
-                if (see0) o[nn][e] += f;
-                if (see1) o[nn][2 + e] += f;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (see[nt][e]) o[nt][nn][2 * h + e] += f;
               }
           }
           __syncwarp();
@@ -361,34 +385,40 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
       __syncwarp();
       float probe = 0.0f;
 #pragma unroll
-      for (int nn = 0; nn < DP / 8; ++nn)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) probe = fmaf(o[nn][e], 0.0f, probe);  // NaN if one is not finite
+        for (int nn = 0; nn < DP / 16; ++nn)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) probe = fmaf(o[nt][nn][e], 0.0f, probe);  // NaN if one is not finite
       if (!__any_sync(0xffffffffu, probe != 0.0f)) break;
     }
 
     // join the warps
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-      if ((lane & 3) == 0) join_m[warp][lane / 4 + 8 * half] = m[half], join_l[warp][lane / 4 + 8 * half] = l[half];
-    }
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], w);
+        if (lane < 4) join_m[warp][8 * nt + 2 * lane + e] = m[nt][e], join_l[warp][8 * nt + 2 * lane + e] = l[nt][e];
+      }
     __syncthreads();  // every warp's copies have landed and its stages are free
     float* acc = (float*)pool + warp * ROWS * DP;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = lane / 4 + 8 * half;
-      if (r < rows) {
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * nt + 2 * (lane & 3) + e;
+        if (r >= rows) continue;
         float mm = join_m[0][r];
 #pragma unroll
         for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, join_m[w][r]);
-        const float sc = exp2f(m[half] - (mm == -INFINITY ? 0.0f : mm));
+        const float sc = exp2f(m[nt][e] - (mm == -INFINITY ? 0.0f : mm));
 #pragma unroll
-        for (int nn = 0; nn < DP / 8; ++nn)
-          *(float2*)(acc + r * DP + nn * 8 + 2 * (lane & 3)) = make_float2(o[nn][2 * half] * sc, o[nn][2 * half + 1] * sc);
+        for (int nn = 0; nn < DP / 16; ++nn)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) acc[r * DP + nn * 16 + 8 * h + (lane >> 2)] = o[nt][nn][2 * h + e] * sc;
       }
-    }
     __syncthreads();
     const bool whole = it.kt0 == 0 && it.kt1 == it.tiles;
     float* slot = slot_of(a, 2 * blockIdx.x + (it.kt0 == 0 ? 1 : 0), ROWS);
@@ -417,21 +447,27 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(Args a) {
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int NT>
 int launch(Args& a, cudaStream_t st) {
   const size_t smem = Smem<DP>::POOL + 4 * (size_t)(a.t.batch + 1);
   static bool ready[64];  // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
-    e = cudaFuncSetAttribute(few_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(few_rows_kernel<T, DP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Smem<DP>::POOL + 4 * (EA_TREE_MAX_SEQS + 1));
     if (e == cudaSuccess && dev < 64) ready[dev] = true;
   }
   if (e != cudaSuccess) return cuda_rc(e);
-  e = launch_early(few_rows_kernel<T, DP>, a.workers, THREADS, smem, st, a);
+  e = launch_early(few_rows_kernel<T, DP, NT>, a.workers, THREADS, smem, st, a);
   if (e != cudaSuccess) return cuda_rc(e);
-  return launch_combine<T, ROWS, KT, EXTRA>(a, st);
+  return launch_combine<T, 8 * NT, KT, EXTRA>(a, st);
+}
+
+template <typename T>
+int launch_few(Args& a, int rows, cudaStream_t st) {
+  if (a.dp == 64) return rows == 8 ? launch<T, 64, 1>(a, st) : launch<T, 64, 2>(a, st);
+  return rows == 8 ? launch<T, 128, 1>(a, st) : launch<T, 128, 2>(a, st);
 }
 
 // Most units a call can have, from the sizes the host knows.
@@ -452,12 +488,12 @@ int check(const ea_tree_attention_t* t) {
   if (t->d % 8 || t->d > 128) return fail(-9, "tree_attention: d is no multiple of 8 up to 128");
   if (t->dtype != EA_BF16 && t->dtype != EA_FP16) return fail(-9, "tree_attention: element type is neither bf16 nor fp16");
   if (t->tokens * t->q_heads >= (1ll << 31) || (int64_t)t->max_pages * t->page_size >= (1ll << 31) ||
-      most_units(*t, ROWS, KT) >= (1ll << 31))
+      most_units(*t, 8, KT) >= (1ll << 31))
     return fail(-1, "tree_attention: too many tokens or keys");
   return 0;
 }
 
-// Which kernel, by the query rows per sequence and kv head: at most 16 (few_rows_kernel), below 512 the tensor-core
+// Which kernel, by the query rows per sequence and kv head: at most 8 or 16 (few_rows_kernel), below 512 the tensor-core
 // kernel with 128-row items, else with 256-row items, which take half the traffic from L2 but keep one of two slots
 // idle where an item has 128 rows or fewer (2048 rows: 345 us against 370 us; 7 to 231 rows: 73 us against 68 us).
 // max_new is a hint, so any choice is right for any lengths.
@@ -466,7 +502,7 @@ struct Choice {
 };
 Choice choose(const ea_tree_attention_t& t) {
   const int64_t rows = (int64_t)(t.max_new > 0 ? t.max_new : 1) * (t.q_heads / t.kv_heads);
-  if (rows <= ROWS || t.batch > MANY_MAX_SEQS) return {ROWS, KT, 2};
+  if (rows <= MAX_ROWS || t.batch > MANY_MAX_SEQS) return {rows <= 8 ? 8 : MAX_ROWS, KT, 2};
   return {rows < 512 ? 128 : 256, 128, 1};
 }
 int workers_for(const ea_tree_attention_t& t, const Choice& c) {
@@ -508,8 +544,6 @@ extern "C" int ea_tree_attention_cuda(const ea_tree_attention_t* t, void* stream
   const tree::Choice c = tree::choose(*t);
   a.workers = tree::workers_for(*t, c);
   cudaStream_t st = (cudaStream_t)stream;
-  if (c.rows > tree::ROWS) return tree::launch_many(a, c.rows == 256, st);
-  if (t->dtype == EA_BF16)
-    return a.dp == 64 ? tree::launch<__nv_bfloat16, 64>(a, st) : tree::launch<__nv_bfloat16, 128>(a, st);
-  return a.dp == 64 ? tree::launch<__half, 64>(a, st) : tree::launch<__half, 128>(a, st);
+  if (c.rows > tree::MAX_ROWS) return tree::launch_many(a, c.rows == 256, st);
+  return t->dtype == EA_BF16 ? tree::launch_few<__nv_bfloat16>(a, c.rows, st) : tree::launch_few<__half>(a, c.rows, st);
 }

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(Args a) {
 template <typename T, int ROWS, int KT, int EXTRA>
 int launch_combine(const Args& a, cudaStream_t st) {
   if (a.workers <= 1) return 0;
-  return cuda_rc(launch_early(combine_kernel<T, ROWS, KT, EXTRA>, dim3((unsigned)a.workers, ROWS / 16), COMBINE_THREADS,
+  return cuda_rc(launch_early(combine_kernel<T, ROWS, KT, EXTRA>, dim3((unsigned)a.workers, (ROWS + 15) / 16), COMBINE_THREADS,
                               4 * (size_t)(a.t.batch + 1), st, a));
 }
 
