@@ -25,18 +25,6 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-// A piece, which is read once: evict-first loads for 32-bit elements (19.6 -> 17.4 us for 4099 tokens of 32 heads of 96);
-// for 16-bit elements plain loads are faster (54 us against 56 us for 16927 tokens into the cache).
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> load_piece(const T* p) {
-  if constexpr (sizeof(T) == 4 && VEC == 4) {
-    const float4 w = __ldcs((const float4*)p);
-    return {{w.x, w.y, w.z, w.w}};
-  } else {
-    return *(const Pack<T, VEC>*)p;
-  }
-}
-
 // Keeps the compiler from widening a piece's numbers before this point, which would double the registers it takes
 // across the barrier.
 template <typename T, int VEC>
@@ -120,8 +108,8 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : ITEMS == 4 ? 3 : 
       src = (const T*)a.v + tok * a.v_stride + (h - nk) * a.v_head_stride;
       dst[i] = (T*)a.v_cache + v_row + (h - nk) * a.v_cache_head_stride + o;
     }
-    x[i] = load_piece<T, VEC>(src + o);
-    if (turn) y[i] = load_piece<T, VEC>(src + o + apart);
+    x[i] = *(const P*)(src + o);
+    if (turn) y[i] = *(const P*)(src + o + apart);
   }
 
   for (uint32_t e = threadIdx.x; e < (uint32_t)(toks * half); e += THREADS) {
