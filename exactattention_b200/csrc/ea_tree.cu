@@ -6,8 +6,8 @@
 // keys are the M side of the scores, channels the M side of the outputs, rows the N side of both, so few rows
 // cost few instructions. With rows on the M side two rows cost what sixteen do: 64 sequences of 4096 to 32768 keys,
 // 2 rows, d = 128 took 776 us in bursts and 860 us in a long loop, where the 1000 W limit lowered the SM clock to 1.7 to
-// 1.85 GHz; this way round takes 737 us and 790 us. Sixteen rows lose to the turning over of the weights: 895 us before,
-// 915 us now in a long loop (d = 128). A warp owns 16 of a tile's 64 keys with a running maximum, sum and output of its
+// 1.85 GHz; this way round takes 737 us and 790 us. Sixteen rows, which have the same products either way and turn
+// their weights over on top, pay for it: 895 us before, 915 us now in a long loop (d = 128). A warp owns 16 of a tile's 64 keys with a running maximum, sum and output of its
 // own, so the warps of a block stream their keys without waiting for one another and join once per item. Bound by HBM: a
 // 16-key slice is 8 KB of K and V at d = 128, for which an SM has about 350 cycles at the measured copy rate, and
 // needs 24 matrix instructions (8 rows; 48 for 16) and 16 ldmatrix of its four sub-partitions.
@@ -317,10 +317,12 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(Args a) {
               float mx = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][2 + e]));
 #pragma unroll
               for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+              if (!(mx > m[nt][e] + LAZY)) mx = m[nt][e];  // another row's score: this row's bits do not depend on it
               const float scale = ex2(m[nt][e] - (mx == -INFINITY ? 0.0f : mx));
-              m[nt][e] = mx, l[nt][e] *= scale;
+              const float f = m[nt][e] == mx ? 1.0f : scale;
+              m[nt][e] = mx, l[nt][e] *= f;
 #pragma unroll
-              for (int nn = 0; nn < DP / 16; ++nn) o[nt][nn][e] *= scale, o[nt][nn][2 + e] *= scale;
+              for (int nn = 0; nn < DP / 16; ++nn) o[nt][nn][e] *= f, o[nt][nn][2 + e] *= f;
             }
         }
 #pragma unroll

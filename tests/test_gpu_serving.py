@@ -253,6 +253,31 @@ def test_tree_attention_flat_and_sharp_scores(spread):
     check_attention(attention_inputs([400, 3], [3, 30], 8, 2, 128, 16, torch.bfloat16, spread=spread))
 
 
+@pytest.mark.parametrize("step", [0.02, 0.6, 20.0, -0.6])
+@pytest.mark.parametrize("new,hk", [(1, 4), (1, 1), (5, 4), (40, 4)])
+def test_tree_attention_scores_that_grow_along_the_keys(new, hk, step):
+    """A row's reference moves seldom, or with every key, or never again."""
+    x = attention_inputs([500], [new], 8, hk, 64, 16, torch.float16)
+    at = torch.zeros(x["k_cache"].shape[0] * 16, device=DEV)
+    n = x["page_table"].shape[1] * 16
+    slots = (x["page_table"][0].long()[:, None] * 16 + torch.arange(16, device=DEV)).reshape(-1)
+    at[slots] = step * torch.arange(n, device=DEV, dtype=torch.float32)
+    x["q"][..., 0] = 1.0
+    x["k_cache"][..., 0] = (at.reshape(-1, 16)[:, None, :] / x["alpha"]).clamp(-6e4, 6e4).half()
+    check_attention(x)
+
+
+@pytest.mark.parametrize("new,hk", [(1, 4), (1, 1), (5, 4), (40, 4), (300, 4)])
+def test_tree_attention_rows_do_not_depend_on_one_another(new, hk):
+    x = attention_inputs([300], [new], 8, hk, 128, 16, torch.bfloat16)
+    want = serving.tree_attention(**x)
+    q = x["q"].clone()
+    q[1:] *= 8
+    q[:, 1::2] *= 8
+    got = serving.tree_attention(**dict(x, q=q))
+    assert torch.equal(got[0, ::2], want[0, ::2])
+
+
 @pytest.mark.parametrize("new", [2, 30, 90])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_tree_attention_values_that_are_not_seen(new, dtype):
