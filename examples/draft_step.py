@@ -1,5 +1,5 @@
 """One step of a speculative decoding server over draft trees, on synthetic data: the serving operators together,
-and the certified attention over the same paged cache as the judge of the draft model's attention.
+and the certified attention over the same paged cache as the check on the draft model's attention.
 
     python examples/draft_step.py            # prints what each part did
 
