@@ -4,7 +4,7 @@
 // the few tokens that penalties or biases change are corrected afterwards. Which these are is kept in 32-bit words:
 //   bits 0-19 how often the token was generated, bits 20-30 which bias entry it has first
 //   (EA_LOGITS_MAX_BIASES - entry, 0: none), bit 31 whether the prompt holds it.
-// The words are integers, so the order of the atomics cannot change them. Whoever finds a word (or a table entry) fresh
+// The words are integers, so the order of the atomics cannot change them. Who finds a word (or a table entry) fresh
 // puts it on a list, from which the corrections are done with full warps.
 //   Many rows: dense_kernel streams all rows through; sparse_kernel, a block a row, collects the row's history, path and
 //   biases in a hash table in shared memory and corrects their tokens. It is launched to start while the dense kernel
@@ -14,7 +14,9 @@
 //   row of 32000 tokens).
 // Measured otherwise for 256 rows of 131072 16-bit logits with 4096 history entries: the chunk kernel for all 68 us; with
 // a cluster of blocks sharing the scan through distributed shared memory 99 us; with a kernel before it that sorts
-// every row's history by chunk 60 us.
+// every row's history by chunk 60 us; dense and sparse kernel 54 us, of which the dense one alone takes 23 us. With the
+// dense kernel as one wave that leaves room for the sparse one's blocks from the start they take 71 to 85 us together: the
+// scattered reads get into the way of the stream. An atomic for every new list entry instead of one a warp: 56 us.
 #include <type_traits>
 
 #include "ea_serving.cuh"
@@ -196,21 +198,30 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t 
   // One pass where the lists fit; else as many as the vocabulary needs, pass p taking the tokens that are p modulo
   // their number, so that no pass can overfill the table.
   const uint32_t fill = slots / 4 * 3, passes = n + n_bias <= (int)fill ? 1u : (vocab + fill - 1) / fill;
-  // The word of token t. The table never fills up; the bound on the search is for safety.
-  const auto word_of = [&](uint32_t t) -> uint32_t* {
+  // The entry of token t, and whether it is new. The table never fills up; the bound on the search is for safety.
+  const auto entry_of = [&](uint32_t t, bool& fresh) -> uint32_t {
     uint32_t h = (t * 2654435761u) >> shift;
     for (int i = 0; i < slots; ++i, h = (h + 1) & (uint32_t)(slots - 1)) {
       uint32_t k = keys[h];
       if (k == 0) {
         k = atomicCAS(keys + h, 0u, t + 1);
         if (k == 0) {
-          list[atomicAdd(&listed, 1)] = (uint16_t)h;
+          fresh = true;
           break;
         }
       }
       if (k == t + 1) break;
     }
-    return words + h;
+    return h;
+  };
+  // Puts the new entries of a warp on the list, with one atomic for all of them.
+  const auto append = [&](uint32_t h, bool fresh) {
+    const uint32_t who = __ballot_sync(0xffffffffu, fresh);
+    if (!who) return;
+    int at = 0;
+    if ((tid & 31) == 0) at = atomicAdd(&listed, __popc(who));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << (tid & 31)) - 1));
+    if (fresh) list[at] = (uint16_t)h;
   };
   for (uint32_t pass = 0; pass < passes; ++pass) {
     const auto mine = [&](uint32_t t) { return t < vocab && (passes == 1 || t % passes == pass); };
@@ -227,19 +238,28 @@ __global__ void __launch_bounds__(THREADS, 2) sparse_kernel(ea_process_logits_t 
       }
 #pragma unroll
       for (int e = 0; e < BATCH; ++e) {
-        if (!mine(tok[e])) continue;
-        uint32_t* w = word_of(tok[e]);
-        if (first + e * THREADS + tid < r.n_prompt) atomicOr(w, PROMPT);
-        else atomicAdd(w, 1u);
+        uint32_t h = 0;
+        bool fresh = false;
+        if (mine(tok[e])) {
+          h = entry_of(tok[e], fresh);
+          if (first + e * THREADS + tid < r.n_prompt) atomicOr(words + h, PROMPT);
+          else atomicAdd(words + h, 1u);
+        }
+        append(h, fresh);
       }
     }
     __syncthreads();
-    for (int e = tid; e < n_bias; e += THREADS) {
-      const uint32_t t = (uint32_t)ids[e];
-      if (!mine(t)) continue;
-      uint32_t* w = word_of(t);
-      const uint32_t old = atomicMax(w, (*w & (PROMPT | COUNT)) | (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT);
-      if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
+    for (int e0 = 0; e0 < n_bias; e0 += THREADS) {  // whole warps come here
+      const int e = e0 + tid;
+      const uint32_t t = e < n_bias ? (uint32_t)ids[e] : EMPTY;
+      uint32_t h = 0;
+      bool fresh = false;
+      if (mine(t)) {
+        h = entry_of(t, fresh);
+        const uint32_t old = atomicMax(words + h, (words[h] & (PROMPT | COUNT)) | (uint32_t)(EA_LOGITS_MAX_BIASES - e) << CODE_SHIFT);
+        if ((old >> CODE_SHIFT) & 0x7FFu) dup = 1;
+      }
+      append(h, fresh);
     }
     __syncthreads();
     const int used = listed;

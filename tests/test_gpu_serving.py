@@ -438,6 +438,33 @@ def test_process_logits_parts_and_rows_without_a_sequence():
     assert e.shape == (0, 5003)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,pad", [(650, 37, 0), (611, 1000, 8), (700, 4099, 0), (90, 131075, 5)])
+@pytest.mark.parametrize("tree", [None, "chain", "tree"])
+def test_process_logits_many_rows(dtype, rows, vocab, pad, tree):
+    """More blocks than the kernel for few rows is taken for."""
+    check_logits(*logits_inputs(rows, vocab, 11, dtype, seed=vocab, tree=tree, pad=pad))
+
+
+@pytest.mark.parametrize("parts", [("history", "history_lens", "frequency"), ("bias_ids", "bias_values"),
+                                   ("allowed_bits", "mask_rows"), ("history", "history_lens", "presence", "allowed_bits", "mask_rows")])
+def test_process_logits_many_rows_parts(parts):
+    x, kw = logits_inputs(660, 2003, 660, torch.float32)
+    kw["row_seq"][::7] = -1
+    kw["row_seq"][3] = 1 << 30
+    check_logits(x, {k: kw[k] for k in parts + ("row_seq",)})
+
+
+@pytest.mark.parametrize("rows,vocab,hist", [(70, 131075, 9000), (600, 601, 1500), (50, 200000, 13000)])
+def test_process_logits_many_rows_long_histories(rows, vocab, hist):
+    """Lists that fit the table, that are many times the vocabulary, and that take several passes."""
+    x, kw = logits_inputs(rows, vocab, 5, torch.bfloat16, hist=hist, nb=400)
+    check_logits(x, kw)
+    x, kw = logits_inputs(rows, vocab, 5, torch.bfloat16, hist=hist, nb=40, grammar=False)
+    kw["bias_ids"][:] = kw["bias_ids"] % 7  # every id several times
+    check_logits(x, kw)
+
+
 def test_process_logits_same_bias_twice_adds_in_order():
     x, kw = logits_inputs(2, 300, 2, torch.float32, nb=40, grammar=False)
     kw["bias_ids"][:] = kw["bias_ids"] % 7  # every id several times
