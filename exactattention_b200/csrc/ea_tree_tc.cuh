@@ -20,7 +20,7 @@
 // random sign, about the rounding of the output itself); their sum takes them unrounded.
 // Measured on one B200: 16 trees of 17 to 64 nodes over 1K to 15K keys, 16 / 8 heads of 128, 144 us in bursts and 155 us in
 // a long loop (545 MB of keys and values: 83 us at the copy rate); four chunks of 256 tokens behind 16K keys, 32 / 4
-// heads, 333 us and, with the SM clock lowered by the 1000 W limit, 383 us (277 GFLOP: 170 us at
+// heads, 333 us in bursts and 383 us in a long loop (277 GFLOP: 170 us at
 // the measured bf16 rate; the tensor pipe is active 42% of the time). A slot's cycle at 128 x 128 x 128 is what bounds it:
 // some 1900 cycles for the weights, 400 to store them and hand them over, 1750 for the issue of the 16 products beside
 // busy softmax warps, 400 until the scores are seen, 4800 in all for both slots' tiles.
