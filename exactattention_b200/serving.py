@@ -133,7 +133,8 @@ def tree_attention(q, k_cache, v_cache, page_table, seq_lens, q_start, alpha, *,
     A token sees its sequence's earlier keys and, of the step's tokens, those whose bit is set in its row
     of tree_mask ((tokens, words) int32, see `tree_mask`); None: itself and the ones before it. Weights are
     2^(alpha q.k) (formats.default_alpha), as in `cuda.launch`. max_new (the most tokens of any sequence)
-    only tunes tile sizes. Rows past q_start[batch] are not written. Returns out (tokens, q_heads, d), and
+    only tunes tile sizes. Rows past q_start[batch] are not written. Rows of q, of the caches and of `out`
+    (contiguous) start on 16-byte boundaries. Returns out (tokens, q_heads, d), and
     with return_lse the log2 of the weights' sums (tokens, q_heads) float32; a row that sees no key gives 0
     and -inf. Values of keys that a row does not see cannot reach it. The result is not certified: it is the
     draft model's attention, accurate to its type's rounding."""

@@ -94,7 +94,8 @@ int ea_rope_cuda(const ea_rope_t* args, void* stream);
  * With w_j = 2^(alpha q . k_j) over the visible keys: out = sum w v / sum w, lse = log2 sum w (NULL: not
  * written); a row that sees no key gives 0 and -inf. Head h reads kv head h / (q_heads / kv_heads).
  * What a row does not see cannot reach its output, NaN and infinities included.
- * bf16 or fp16 (q, caches and out alike), d a multiple of 8 up to 128, 16-byte aligned rows.
+ * bf16 or fp16 (q, caches and out alike), d a multiple of 8 up to 128, rows on 16-byte boundaries (-9
+ * otherwise).
  * max_new: the most tokens any sequence has in this step (a hint: it sizes tiles, not results).
  * workspace: ea_tree_attention_workspace(args) bytes, 16-byte aligned, any contents; calls that
  * may overlap need workspaces of their own. Page ids outside 0 .. num_pages - 1 are read as keys no

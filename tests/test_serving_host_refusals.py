@@ -1,0 +1,24 @@
+"""What the serving operators refuse on the host, before any launch, beyond test_serving_host.py."""
+
+import ctypes
+
+import pytest
+
+from exactattention_b200 import _lib
+
+
+@pytest.mark.parametrize("off", [2, 4, 8, 24])
+@pytest.mark.parametrize("name", ["q", "k_cache", "v_cache", "out", "workspace"])
+def test_tree_attention_refuses_rows_off_16_byte_boundaries(cuda_lib, name, off):
+    """The kernels load and store rows 8 and 16 bytes at a time. The addresses are made up: the call has to come
+    back without a launch."""
+    t = _lib.TreeAttentionArgs()
+    t.tokens, t.batch, t.q_heads, t.kv_heads, t.d, t.page_size, t.max_pages, t.num_pages, t.max_new = 40, 1, 4, 2, 64, 16, 4, 4, 40
+    t.q_stride, t.q_head_stride = 256, 64
+    t.k_page_stride, t.k_head_stride, t.k_row_stride = 2048, 1024, 64
+    t.v_page_stride, t.v_head_stride, t.v_row_stride = 2048, 1024, 64
+    for i, f in enumerate(("q", "k_cache", "v_cache", "page_table", "seq_lens", "q_start", "out", "workspace")):
+        setattr(t, f, (i + 1) << 20)
+    setattr(t, name, getattr(t, name) + off)
+    assert cuda_lib.ea_tree_attention_cuda(ctypes.byref(t), None) == -9
+    assert b"16-byte" in cuda_lib.ea_serving_last_error()
