@@ -12,9 +12,9 @@
 // 16-key slice is 8 KB of K and V at d = 128, for which an SM has about 350 cycles at the measured copy rate, and
 // needs 24 matrix instructions (8 rows; 48 for 16) and 16 ldmatrix of its four sub-partitions.
 // Weights enter P.V as a pair of 16-bit numbers, their rounding and its remainder (relative error 2^-17 for bf16
-// instead of 2^-9), which is 8 of those 24 instructions: the tensor pipe has the room.
-#include <type_traits>
-
+// instead of 2^-9; for fp16 2^-22 or 2^-36 of the row's largest weight, whichever is more), which is 8 of those 24
+// instructions: the tensor pipe has the room. A row's reference moves seldom (Reference in ea_tree.cuh), so most slices need no
+// reduction over lanes.
 #include "ea_tree.cuh"
 
 namespace ea {
@@ -24,10 +24,6 @@ namespace tree {
 namespace {
 
 constexpr int MAX_ROWS = 16, WARPS = 4, KT = 16 * WARPS, THREADS = 32 * WARPS, STAGES = 3, EXTRA = 1;
-
-// A row's reference moves only when a score passes it by more than this (in powers of two): the weights are then at
-// most 256, which both types hold with the same relative error, and most slices need no reduction over lanes.
-constexpr float LAZY = 8.0f;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -307,20 +303,21 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(Args a) {
               const int kk = (lane >> 2) + 8 * (e >> 1);
               if (!sees(a, it, tok[nt][e & 1], key0 + kk, (okm >> kk) & 1)) s[nt][e] = -INFINITY;
             }
-            grows |= s[nt][e] > m[nt][e & 1] + LAZY;
+            grows |= Reference<T>::passed(s[nt][e], m[nt][e & 1]);
           }
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float mx = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][2 + e]));
+              float mx = fmaxf(s[nt][e], s[nt][2 + e]);
 #pragma unroll
               for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-              if (!(mx > m[nt][e] + LAZY)) mx = m[nt][e];  // another row's score: this row's bits do not depend on it
-              const float scale = ex2(m[nt][e] - (mx == -INFINITY ? 0.0f : mx));
-              const float f = m[nt][e] == mx ? 1.0f : scale;
-              m[nt][e] = mx, l[nt][e] *= f;
+              // where another row's score passed, this row keeps its reference: its bits do not depend on others
+              const float to = Reference<T>::passed(mx, m[nt][e]) ? mx - Reference<T>::DOWN : m[nt][e];
+              const float scale = ex2(m[nt][e] - (to == -INFINITY ? 0.0f : to));
+              const float f = m[nt][e] == to ? 1.0f : scale;
+              m[nt][e] = to, l[nt][e] *= f;
 #pragma unroll
               for (int nn = 0; nn < DP / 16; ++nn) o[nt][nn][e] *= f, o[nt][nn][2 + e] *= f;
             }

@@ -7,6 +7,8 @@
 // tile) that crosses shares leaves one partial (row maximum, row sum, unnormalised output) per share,
 // which the block of the combine kernel that belongs to the item's first share adds up in share order.
 #pragma once
+#include <type_traits>
+
 #include "ea_serving.cuh"
 
 namespace ea {
@@ -19,6 +21,22 @@ struct Args {
   int group;     // query heads per kv head
   int workers;   // blocks that share the units
   int dp;        // channels of a partial: d rounded up
+};
+
+// The reference m of a row's weights 2^(s - m), in powers of two. When it moves it is put DOWN below the largest score seen;
+// it moves only when a score passes m + DOWN by more than LAZY, so that most tiles rescale nothing. Sums, outputs, partials
+// and the log-sum-exp all refer to m, whatever it is.
+// bf16 has binary32's exponents: a weight keeps its relative error at any size, and DOWN is 0. fp16 loses bits below
+// 2^-14 and everything below 2^-25, where the long tail behind one dominant key lies: DOWN + LAZY = 15 uses its range up to
+// 2^15, so that the product takes a weight to within 2^-36 of the row's largest (the sum takes it unrounded).
+template <typename T>
+struct Reference {
+  static constexpr bool HALF = std::is_same<T, __half>::value;
+  static constexpr float DOWN = HALF ? 11.0f : 0.0f, LAZY = HALF ? 4.0f : 8.0f;
+  // Whether a score moves m. In fp16 by the difference, which is what the weight will be: m + 15 may round up.
+  static __device__ __forceinline__ bool passed(float score, float m) {
+    return HALF ? score - m > DOWN + LAZY : score > m + LAZY;
+  }
 };
 
 struct Item {

@@ -14,10 +14,10 @@
 // cycles of the tensor pipe and the 16384 exponentials 1024 cycles of the special-function pipe.
 // The MMA thread issues PV(t) and then QK of the slot's next tile, so one arrival per cycle tells the slot that its
 // scores are there and that O is at rest: the rescale of O needs no wait of its own. It happens only when a row's
-// maximum grew by more than 8 (weights stay below 2^8, far from any overflow, and nothing is lost: the sum and O
-// share the reference).
-// Weights are rounded to the cache's type for the product (relative error 2^-9 for bf16, 2^-12 for fp16, of
-// random sign, about the rounding of the output itself); their sum takes them unrounded.
+// reference moves (Reference in ea_tree.cuh; the sum and O share it).
+// Weights are rounded to the cache's type for the product (relative error 2^-9 for bf16; 2^-12 for fp16 down to 2^-25 of the
+// row's largest weight, below that 2^-36 of the largest; of random sign, about the rounding of the output itself);
+// their sum takes them unrounded.
 // Measured on one B200: 16 trees of 17 to 64 nodes over 1K to 15K keys, 16 / 8 heads of 128, 144 us in bursts and 155 us in
 // a long loop (545 MB of keys and values: 83 us at the copy rate); four chunks of 256 tokens behind 16K keys, 32 / 4
 // heads, 333 us in bursts and 383 us in a long loop (277 GFLOP: 170 us at
@@ -597,8 +597,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           // One pass in the common case (a first pass for the maximum alone cost 500 cycles of a tile's 2650; holding the whole
           // tile's scores in registers spilled): the weights against the maximum so far, while the tile's own is taken.
-          // They are stored, over the scores, only if no row's maximum grew by more than 8; else O is rescaled and
-          // a second pass computes them anew. A slot's first tile takes its maximum before.
+          // They are stored, over the scores, only if no row's reference moved; else O is rescaled and a second pass
+          // computes them anew. A slot's first tile takes its maximum before.
           uint32_t u[2][16], p[KT / 2];
           float2 sum[2];
           float mx[2] = {-INFINITY, -INFINITY};
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int e = 0; e < 8; ++e) mx[e & 1] = max3(mx[e & 1], __uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
             });
-            m = fmaxf(mx[0], mx[1]) * scale_s;
+            m = fmaxf(mx[0], mx[1]) * scale_s - Reference<T>::DOWN;
           }
           for (int pass = 0; pass < 2; ++pass) {
             const float ref = m == -INFINITY ? 0.0f : m;
@@ -638,10 +638,10 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
             });
             const float top = fmaxf(mx[0], mx[1]) * scale_s;
-            const bool grow = top > m + 8.0f || (m == -INFINITY && top != -INFINITY);
+            const bool grow = Reference<T>::passed(top, m);
             if (!__any_sync(0xffffffffu, grow)) break;
-            const float f = grow ? (m == -INFINITY ? 0.0f : ex2(m - top)) : 1.0f;
-            if (grow) m = top;
+            const float to = top - Reference<T>::DOWN, f = grow ? (m == -INFINITY ? 0.0f : ex2(m - to)) : 1.0f;
+            if (grow) m = to;
             l *= f;
             if (i > 0) {
 #pragma unroll 1

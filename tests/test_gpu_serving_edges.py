@@ -4,8 +4,9 @@ that one of the kernels or its host side once got wrong."""
 import pytest
 import torch
 
+import serving_ref as ref
 from exactattention_b200 import serving
-from test_gpu_serving import DEV, attention_inputs
+from test_gpu_serving import DEV, attention_inputs, check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +23,51 @@ def test_tree_attention_out_off_a_16_byte_boundary_is_refused(new):
     out = buf[8:].view(want.shape)
     assert serving.tree_attention(**x, out=out) is out and torch.equal(out, want)
     assert not bool(buf[:8].any())
+
+
+@pytest.mark.parametrize("tail", [-26.0, -30.0])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("seqs,new,hq,hk", [(24, 1, 32, 16), (12, 24, 32, 16), (4, 130, 64, 16)])
+def test_tree_attention_long_tail_behind_dominant_keys(dtype, seqs, new, hq, hk, tail):
+    """A few keys with values of 0 dominate the sum, and thousands some 2^26 below them make the output: fp16 holds
+    no weight below 2^-25 of its reference. The dominant keys lie where every warp, and every slot of the tensor-core
+    kernel, has one; there are enough items for most to lie in one share."""
+    d, ctx = 32, 8192
+    x = attention_inputs([ctx] * seqs, [new] * seqs, hq, hk, d, 16, dtype, mask="chain")
+    g = torch.Generator(device=DEV).manual_seed(1)
+    kc, vc = x["k_cache"], x["v_cache"]
+    x["q"].zero_()
+    x["q"][..., 0] = 1
+    kc.zero_()
+    kc[..., 0] = ((tail + 4 * torch.rand(kc.shape[:3], generator=g, device=DEV) - 2) / x["alpha"]).to(dtype)
+    vc.copy_(64 * (1 + 0.25 * torch.randn(vc.shape, generator=g, device=DEV)))
+    for key in (0, 16, 32, 48, 128):
+        page = x["page_table"][:, key // 16].long()
+        kc[page, :, key % 16], vc[page, :, key % 16] = 0, 0
+    check_attention(x, max_new=new)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("size,step", [(2.0**24, 4.0), (2.0**24, 16.0), (2.0**26, 8.0), (2.0**26, 16.0), (2.0**29, 64.0)])
+def test_tree_attention_huge_scores_that_grow(dtype, new, size, step):
+    """Scores of a size at which 32-bit numbers are as far apart as the distance at which a row's reference moves: no
+    weight may overflow its type. Every score is size + step * (0 .. 3), exact in 32 bits, so only the weights' and the
+    output's roundings are left: 2^-14 for exp2 and the sums, half a unit of the type for each of the two."""
+    x = attention_inputs([300], [new], 4, 2, 16, 16, dtype, mask="chain")
+    q, kc, vc = x["q"], x["k_cache"], x["v_cache"]
+    q.zero_(), kc.zero_()
+    q[..., 0], q[..., 1] = 2.0**12, 1.0
+    n = 300 + new
+    key = torch.arange(n, device=DEV)
+    page, row = x["page_table"][0].long()[key // 16], key % 16
+    level = (4 * key // n).double()  # grows along the keys
+    kc[page, :, row, 0] = size / 2.0**14
+    kc[page, :, row, 1] = (step / 4 * level).to(dtype)[:, None]
+    out, lse = serving.tree_attention(**dict(x, alpha=4.0), return_lse=True)
+    v = vc[page, :, row].double()  # (key, kv head, d)
+    w = torch.exp2(step * (level - 3))[None] * (key[None] <= 300 + torch.arange(new, device=DEV)[:, None])
+    o, mag = (torch.einsum("tn,nhd->thd", w, y).repeat_interleave(2, 1) / w.sum(1)[:, None, None] for y in (v, v.abs()))
+    u = ref.HALF_ULP[dtype]
+    ref.assert_within(out, o, u * o.abs() + (u + 2.0**-14) * mag + ref.TINY[dtype])
+    assert bool(((lse - size).abs() <= 3 * step + 16 + size * 2.0**-23).all())
