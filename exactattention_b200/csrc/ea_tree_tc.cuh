@@ -266,11 +266,12 @@ __device__ __noinline__ bool clean_row(uint8_t* buf, int row) {
   return any;
 }
 
-// Adds to acc (channels c0 ..) the infinities and NaN of the values of drafted keys first .. last - 1 that token i sees.
+// Adds to acc (channels c0 ..) the infinities and NaN of the values of keys first .. last - 1 that token i sees, as far as
+// their tiles were cleaned: from the tile on that holds the first drafted key.
 template <typename T, int N>
 __device__ __noinline__ void add_not_finite(const Args& a, const Item& it, int i, int first, int last, int c0, float* acc) {
-  for (int k = max(first, it.len - it.new_tokens); k < min(last, it.len); ++k) {
-    if (k < 0 || !((seen_word(a, it, i, k)) & 1)) continue;
+  for (int k = max(first, max(it.len - it.new_tokens, 0) / KT * KT); k < min(last, it.len); ++k) {
+    if (!((seen_word(a, it, i, k)) & 1)) continue;
     const uint32_t col = div_by((uint32_t)k, a.by_page);
     const int page = a.t.page_table[it.b * a.t.table_stride + col];
     if (page < 0 || page >= a.t.num_pages) continue;
@@ -660,7 +661,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
         }
-        // drafted keys: their infinities and NaN may not meet the zero weight of a row that does not see them
+        // Drafted keys, and rows behind the last key: their infinities and NaN may not meet the zero weight of a row
+        // that does not see them. The tile's whole rows are cleaned, earlier keys' too; rows that see them get them back at the end.
         if (key0 + KT > ctx && (!PAIR || slot == 0)) {
           const uint32_t c = first + (PAIR ? 1 + 2 * t : n == 1 ? 1 : 2 + t + min(t, n - 2));
           wait(&sh.full[c % NBUF], (c / NBUF) & 1);

@@ -1,6 +1,8 @@
 """The serving operators on the GPU where they are easily wrong, beyond test_gpu_serving.py: each test holds a case
 that one of the kernels or its host side once got wrong."""
 
+import math
+
 import pytest
 import torch
 
@@ -71,3 +73,14 @@ def test_tree_attention_huge_scores_that_grow(dtype, new, size, step):
     u = ref.HALF_ULP[dtype]
     ref.assert_within(out, o, u * o.abs() + (u + 2.0**-14) * mag + ref.TINY[dtype])
     assert bool(((lse - size).abs() <= 3 * step + 16 + size * 2.0**-23).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("key", [0, 130, 199])
+@pytest.mark.parametrize("new,hq,ps", [(4, 4, 16), (40, 4, 16), (40, 4, 24), (300, 4, 16), (40, 40, 16)])
+def test_tree_attention_infinite_values_beside_the_drafted_keys(dtype, key, new, hq, ps):
+    """A context key in the tile where the drafted keys begin (128 .. 255): every row sees its infinities and NaN."""
+    x = attention_inputs([200], [new], hq, 1, 64, ps, dtype)
+    v = x["v_cache"][x["page_table"][0, key // ps].item(), 0, key % ps]
+    v[:3] = torch.tensor([math.inf, -math.inf, math.nan], device=DEV).to(dtype)
+    check_attention(x)
