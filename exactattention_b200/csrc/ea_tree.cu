@@ -144,9 +144,8 @@ __device__ __forceinline__ void load_slice(const Args& a, const Item& it, int ke
 // Whether query row R of the item (token i of the step) sees key `key`.
 __device__ __forceinline__ bool sees(const Args& a, const Item& it, int i, int key, int page_ok) {
   if (key >= it.len || !page_ok) return false;
-  const int ctx = it.len - it.new_tokens;
-  if (key < ctx) return true;
-  const int j = key - ctx;
+  if (key < it.ctx) return true;
+  const int j = key - it.ctx;
   if (!a.t.tree_mask) return j <= i;
   return (j >> 5) < a.t.mask_words && ((a.t.tree_mask[(int64_t)(it.q0 + i) * a.t.mask_words + (j >> 5)] >> (j & 31)) & 1);
 }
@@ -184,7 +183,6 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(Args a) {
     const Item it = sch.item(a, pos, end);
     pos = it.next;
     if (it.kt0 >= it.kt1) continue;
-    const int ctx = it.len - it.new_tokens;
     const int rows = min(ROWS, it.new_tokens * a.group - it.m * ROWS);
     const int R0 = it.m * ROWS;
 
@@ -291,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 2) few_rows_kernel(Args a) {
             for (int nt = 0; nt < NT; ++nt) mma<T>(s[nt], f, qf[nt][ks][0], qf[nt][ks][1]);
           }
         }
-        const bool masked = key0 + 16 > ctx || okm != 0xFFFFu;
+        const bool masked = key0 + 16 > it.ctx || okm != 0xFFFFu;
         uint32_t hi[NT][2], lo[NT][2];
         bool grows = false;
 #pragma unroll

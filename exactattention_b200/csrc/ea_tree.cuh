@@ -42,17 +42,26 @@ struct Reference {
 struct Item {
   int b, h, m;            // sequence, kv head, row tile
   int q0, new_tokens;     // first token of the step and their number
-  int len;                // keys, the step's own included
+  int len;                // keys that the page table has room for, the step's own included
+  int ctx;                // keys before the step's own
   int kt0, kt1, tiles;    // key tiles of this share (none: kt0 >= kt1), and of the item
   uint32_t next;          // unit after the share's part of the item
 };
 
+// Keys of a sequence, as far as its row of the page table goes: keys past it have no page.
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return (int)min((int64_t)max(a.t.seq_lens[b], 0), (int64_t)a.t.max_pages * a.t.page_size);
 }
+// The step's tokens of a sequence that q has rows for.
 __device__ __forceinline__ void seq_tokens(const Args& a, int b, int& q0, int& n) {
   const int64_t lo = max(a.t.q_start[b], 0), hi = min((int64_t)a.t.q_start[b + 1], a.t.tokens);
   q0 = (int)lo, n = (int)max(hi - lo, (int64_t)0);
+}
+// Keys before the step's own: from the lengths as they are given, whatever the table and q have room for. Negative where the step
+// has more tokens than the sequence keys, but so that key - ctx stays within 32 bits for every key of a tile.
+__device__ __forceinline__ int seq_ctx(const Args& a, int b, int len) {
+  const int64_t n = max((int64_t)a.t.q_start[b + 1] - a.t.q_start[b], (int64_t)0);
+  return (int)max(max(a.t.seq_lens[b], 0) - n, (int64_t)len - 0x7FFFFF00);
 }
 
 template <int ROWS, int KT, int EXTRA>
@@ -111,6 +120,7 @@ struct Schedule {
     it.b = lo;
     seq_tokens(a, lo, it.q0, it.new_tokens);
     it.len = seq_len(a, lo);
+    it.ctx = seq_ctx(a, lo, it.len);
     it.tiles = max(1, (it.len + KT - 1) / KT);
     const uint32_t mt = (uint32_t)((it.new_tokens * a.group + ROWS - 1) / ROWS);
     const uint32_t units = it.tiles + EXTRA, rel = pos - prefix[lo], idx = rel / units, at = rel - idx * units;

@@ -225,7 +225,7 @@ __device__ __forceinline__ uint32_t tile_off(int row, int piece, int rows) {
 
 // Bits of keys k0 .. k0 + 31 that token i of the item sees; tile pages aside.
 __device__ __forceinline__ uint32_t seen_word(const Args& a, const Item& it, int i, int k0) {
-  const int ctx = it.len - it.new_tokens, j0 = k0 - ctx;
+  const int j0 = k0 - it.ctx;
   const auto low = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
   uint32_t bits;
   if (j0 <= -32) {
@@ -270,7 +270,7 @@ __device__ __noinline__ bool clean_row(uint8_t* buf, int row) {
 // their tiles were cleaned: from the tile on that holds the first drafted key.
 template <typename T, int N>
 __device__ __noinline__ void add_not_finite(const Args& a, const Item& it, int i, int first, int last, int c0, float* acc) {
-  for (int k = max(first, max(it.len - it.new_tokens, 0) / KT * KT); k < min(last, it.len); ++k) {
+  for (int k = max(first, max(it.ctx, 0) / KT * KT); k < min(last, it.len); ++k) {
     if (!((seen_word(a, it, i, k)) & 1)) continue;
     const uint32_t col = div_by((uint32_t)k, a.by_page);
     const int page = a.t.page_table[it.b * a.t.table_stride + col];
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Item it = sch.item(a, pos, end);
       pos = it.next;
       if (it.kt0 >= it.kt1) continue;
-      const int n = it.kt1 - it.kt0, ctx = it.len - it.new_tokens;
+      const int n = it.kt1 - it.kt0;
       const int all_rows = it.new_tokens * a.group - it.m * ROWS;
       const int rows = min(TILE, all_rows - (PAIR ? slot * TILE : 0));  // of this slot's tile; may be <= 0 for PAIR
       const int R = it.m * ROWS + (PAIR ? slot * TILE : 0) + min(r, max(rows, 1) - 1);
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         wait(&sh.s_full[slot], ns++ & 1);
         fence_after_sync();
         const uint32_t* ok = sh.page_ok[(first / 2 + t) % PAGE_RING];
-        const bool masked = key0 + KT > ctx || (ok[0] & ok[1] & ok[2] & ok[3]) != 0xFFFFFFFFu;
+        const bool masked = key0 + KT > it.ctx || (ok[0] & ok[1] & ok[2] & ok[3]) != 0xFFFFFFFFu;
         if (warp_rows && alive) {
           uint32_t vis[KT / 32];
           if (masked) {
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         // Drafted keys, and rows behind the last key: their infinities and NaN may not meet the zero weight of a row
         // that does not see them. The tile's whole rows are cleaned, earlier keys' too; rows that see them get them back at the end.
-        if (key0 + KT > ctx && (!PAIR || slot == 0)) {
+        if (key0 + KT > it.ctx && (!PAIR || slot == 0)) {
           const uint32_t c = first + (PAIR ? 1 + 2 * t : n == 1 ? 1 : 2 + t + min(t, n - 2));
           wait(&sh.full[c % NBUF], (c / NBUF) & 1);
           if (alive && clean_row<T, DP>(ring + (c % NBUF) * BUF, r) && key0 + r < it.len) sh.dirty[items & 1][slot] = 1;

@@ -98,8 +98,9 @@ int ea_rope_cuda(const ea_rope_t* args, void* stream);
  * otherwise).
  * max_new: the most tokens any sequence has in this step (a hint: it sizes tiles, not results).
  * workspace: ea_tree_attention_workspace(args) bytes, 16-byte aligned, any contents; calls that
- * may overlap need workspaces of their own. Page ids outside 0 .. num_pages - 1 are read as keys no
- * row sees. Deterministic for equal inputs on one GPU model (no atomics). */
+ * may overlap need workspaces of their own. Page ids outside 0 .. num_pages - 1 and keys past the table's
+ * columns are read as keys no row sees; tokens past `tokens` have no row, but still count among the step's.
+ * Deterministic for equal inputs on one GPU model (no atomics). */
 #define EA_TREE_MAX_SEQS 8192
 typedef struct ea_tree_attention {
   const void* q; /* (tokens, q_heads, d) */

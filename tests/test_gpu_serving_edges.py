@@ -84,3 +84,36 @@ def test_tree_attention_infinite_values_beside_the_drafted_keys(dtype, key, new,
     v = x["v_cache"][x["page_table"][0, key // ps].item(), 0, key % ps]
     v[:3] = torch.tensor([math.inf, -math.inf, math.nan], device=DEV).to(dtype)
     check_attention(x)
+
+
+def reference(x, table=None):
+    return ref.tree_attention(x["q"], x["k_cache"], x["v_cache"], x["page_table"] if table is None else table, x["seq_lens"],
+                              x["q_start"], x["alpha"], None if x["tree_mask"] is None else x["tree_mask"].cpu().numpy())
+
+
+@pytest.mark.parametrize("new,hq", [(6, 2), (40, 4), (300, 4)])
+@pytest.mark.parametrize("mask", ["chain", "tree"])
+@pytest.mark.parametrize("ps", [16, 24])
+def test_tree_attention_sequence_longer_than_its_table(new, hq, mask, ps):
+    """A step that plan_step reports as PLAN_TABLE_FULL: keys past the table's columns are not seen, and which of the others
+    are the step's own still follows from the sequence's length."""
+    x = attention_inputs([10 * ps - new // 2, 20], [new, 3], hq, 1, 64, ps, torch.bfloat16, mask=mask)
+    wide = x["page_table"].clone()
+    wide[0, 10:] = -1
+    o, ls, ob, lb = reference(x, wide)
+    out, lse = serving.tree_attention(**dict(x, page_table=wide[:, :10].contiguous()), return_lse=True)
+    ref.assert_within(out, o, ob)
+    ref.assert_within(lse, ls, lb)
+
+
+@pytest.mark.parametrize("new,hq", [(6, 2), (40, 4), (300, 4)])
+@pytest.mark.parametrize("mask", ["chain", "tree"])
+def test_tree_attention_more_tokens_than_rows(new, hq, mask):
+    """A step that plan_step reports as PLAN_TOO_MANY: the last sequence has tokens without a row of q."""
+    x = attention_inputs([50, 90], [3, new], hq, 1, 64, 16, torch.bfloat16, mask=mask)
+    o, ls, ob, lb = reference(x)
+    n = x["q"].shape[0] - 2
+    y = dict(x, q=x["q"][:n], tree_mask=None if x["tree_mask"] is None else x["tree_mask"][:n].contiguous())
+    out, lse = serving.tree_attention(**y, return_lse=True)
+    ref.assert_within(out, o[:n], ob[:n])
+    ref.assert_within(lse, ls[:n], lb[:n])
