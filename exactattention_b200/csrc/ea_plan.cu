@@ -180,14 +180,19 @@ extern "C" int ea_plan_step_cuda(const ea_plan_step_t* a, void* stream) {
       (a->num_free && !a->free_pages) || (a->max_tokens && (!a->slot_map || !a->positions || !a->token_seq)))
     return fail(-1, "plan_step: a required pointer is NULL");
   if (a->next_free_head == a->free_head) return fail(-1, "plan_step: next_free_head may not be free_head");
-  const size_t smem = 2 * sizeof(int32_t) * (size_t)(a->batch + 1);
-  if (smem > 40 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(plan_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_rc(e);
+  const auto smem_of = [](int batch) { return 2 * (int)sizeof(int32_t) * (batch + 1); };
+  // Room for the largest batch, once per device: the attribute belongs to the device, so a call that set it to its own
+  // batch's would take it from a larger one that another thread is about to launch.
+  static bool ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
+    e = cudaFuncSetAttribute(plan_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(EA_PLAN_MAX_SEQS));
+    if (e == cudaSuccess && dev < 64) ready[dev] = true;
   }
+  if (e != cudaSuccess) return cuda_rc(e);
   const int per_block = THREADS * PER_THREAD;
   const int grid = a->max_tokens > per_block ? (int)(((int64_t)a->max_tokens + per_block - 1) / per_block) : 1;
   const bool vec = (((uintptr_t)a->slot_map | (uintptr_t)a->positions | (uintptr_t)a->token_seq) & 15) == 0;
-  return cuda_rc(launch_early(plan_step_kernel, grid, THREADS, smem, (cudaStream_t)stream, *a, fast_div((uint32_t)a->page_size), vec));
+  return cuda_rc(launch_early(plan_step_kernel, grid, THREADS, smem_of(a->batch), (cudaStream_t)stream, *a, fast_div((uint32_t)a->page_size), vec));
 }

@@ -1,13 +1,15 @@
 """The serving operators on the GPU where they are easily wrong, beyond test_gpu_serving.py: each test holds a case
 that one of the kernels or its host side once got wrong."""
 
+import ctypes
 import math
+import threading
 
 import pytest
 import torch
 
 import serving_ref as ref
-from exactattention_b200 import serving
+from exactattention_b200 import _lib, serving
 from test_gpu_serving import DEV, attention_inputs, check_attention
 
 pytestmark = pytest.mark.gpu
@@ -117,3 +119,33 @@ def test_tree_attention_more_tokens_than_rows(new, hq, mask):
     out, lse = serving.tree_attention(**y, return_lse=True)
     ref.assert_within(out, o[:n], ob[:n])
     ref.assert_within(lse, ls[:n], lb[:n])
+
+
+def test_plan_step_of_two_sizes_from_two_threads():
+    """Large and small batches planned at the same time by two host threads through the C entry (the Python binding holds
+    the interpreter's lock): neither call may take the other's shared memory away."""
+    lib = _lib.load()
+    failed = []
+
+    def work(batch):
+        zeros = torch.zeros(batch, dtype=torch.int32, device=DEV)
+        outs = [torch.zeros(batch + 1, dtype=torch.int32, device=DEV) for _ in range(5)]
+        slots = torch.zeros(8, dtype=torch.int64, device=DEV)
+        a = _lib.PlanStepArgs()
+        a.context_lens = a.new_lens = zeros.data_ptr()
+        a.slot_map, a.positions, a.token_seq = slots.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr()
+        a.q_start, a.seq_lens = outs[2].data_ptr(), outs[3].data_ptr()
+        a.next_free_head, a.status = outs[4].data_ptr(), outs[4].data_ptr() + 4
+        a.batch, a.page_size, a.max_tokens = batch, 16, 8
+        for _ in range(3000):
+            rc = lib.ea_plan_step_cuda(ctypes.byref(a), None)
+            if rc:
+                failed.append((batch, rc, lib.ea_serving_last_error()))
+        torch.cuda.synchronize()
+
+    threads = [threading.Thread(target=work, args=(b,)) for b in (16384, 6000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, (len(failed), failed[0])
