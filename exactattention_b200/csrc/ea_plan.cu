@@ -52,7 +52,8 @@ __device__ __forceinline__ int segment_of(const int32_t* a, int n, int32_t x) {
   return lo;
 }
 
-__device__ __forceinline__ int pages_of(int64_t n, int ps) { return (int)((n + ps - 1) / ps); }
+// 64 bits: a context and its new tokens together may need 2^32 pages of one row.
+__device__ __forceinline__ int64_t pages_of(int64_t n, int ps) { return (n + ps - 1) / ps; }
 
 // Prefix sums saturate at INT32_MAX, so a step with too many tokens still gives ordered sums.
 __device__ __forceinline__ int32_t saturate(int64_t x) { return (int32_t)(x < 0x7FFFFFFF ? x : 0x7FFFFFFF); }
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(THREADS) plan_step_kernel(ea_plan_step_t a, Fa
   for (int b = b0; b < b1; ++b) {
     const int32_t ctx = max(0, a.context_lens[b]), nw = max(0, a.new_lens[b]);
     tok[b] = saturate(pt), frs[b] = saturate(pf);
-    const int need = pages_of((int64_t)ctx + nw, a.page_size);
+    const int64_t need = pages_of((int64_t)ctx + nw, a.page_size);
     pt += nw, pf += need - pages_of(ctx, a.page_size);
     over |= need > a.max_pages;
     if (blockIdx.x == b % gridDim.x) {
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(THREADS) plan_step_kernel(ea_plan_step_t a, Fa
   // fresh pages into the table
   for (int32_t f = blockIdx.x * THREADS + tid; f < fresh; f += gridDim.x * THREADS) {
     const int b = segment_of(frs, a.batch, f);
-    const int col = pages_of(max(0, a.context_lens[b]), a.page_size) + (f - frs[b]);
+    const int64_t col = pages_of(max(0, a.context_lens[b]), a.page_size) + (f - frs[b]);
     const int64_t at = (int64_t)head + f;
     if (col < a.max_pages) a.page_table[b * a.table_stride + col] = at < a.num_free ? a.free_pages[at] : -1;
     if (f > 0x7FFFFFFF - (int32_t)(gridDim.x * THREADS)) break;
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(THREADS) plan_step_kernel(ea_plan_step_t a, Fa
     while (tok[b + 1] <= t) ++b, fetch = true;
     if (fetch) {
       ctx = max(0, a.context_lens[b]), first = tok[b];
-      owned = pages_of(ctx, a.page_size);
+      owned = (int32_t)pages_of(ctx, a.page_size);
       fetch = false;
     }
     const int32_t i = t - first;

@@ -5,12 +5,13 @@ import ctypes
 import math
 import threading
 
+import numpy as np
 import pytest
 import torch
 
 import serving_ref as ref
 from exactattention_b200 import _lib, serving
-from test_gpu_serving import DEV, attention_inputs, check_attention
+from test_gpu_serving import DEV, attention_inputs, check_attention, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +150,14 @@ def test_plan_step_of_two_sizes_from_two_threads():
     for t in threads:
         t.join()
     assert not failed, (len(failed), failed[0])
+
+
+def test_plan_step_page_counts_past_32_bits():
+    """Pages of one row: a context of 2^31 - 1 and one token need 2^31 pages, which no table has."""
+    table = torch.full((2, 3), -1, dtype=torch.int32, device=DEV)
+    big = 2**31 - 1
+    p = serving.plan_step(i32([big, 0]), i32([1, 2]), table, i32(np.arange(8)), 1, 8)
+    assert int(p.status) == serving.PLAN_TABLE_FULL
+    assert p.slot_map.tolist() == [-1, 1, 2, -1, -1, -1, -1, -1] and p.token_seq.tolist() == [0, 1, 1, -1, -1, -1, -1, -1]
+    assert p.q_start.tolist() == [0, 1, 3] and p.seq_lens.tolist() == [big, 2] and int(p.free_head) == 3
+    assert table.tolist() == [[-1, -1, -1], [1, 2, -1]]
