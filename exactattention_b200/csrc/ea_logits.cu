@@ -467,8 +467,8 @@ extern "C" int ea_process_logits_cuda(const ea_process_logits_t* a, void* stream
   if (!a || a->rows < 0 || a->vocab < 0 || a->batch < 0 || a->max_history < 0 || a->num_biases < 0 || a->num_masks < 0 ||
       a->tree_words < 0)
     return fail(-1, "process_logits: negative size");
-  if (a->max_history > EA_LOGITS_MAX_HISTORY || a->num_biases > EA_LOGITS_MAX_BIASES || a->vocab > (1 << 30))
-    return fail(-1, "process_logits: history, biases or vocabulary above their limits");
+  if (a->batch > EA_LOGITS_MAX_SEQS || a->max_history > EA_LOGITS_MAX_HISTORY || a->num_biases > EA_LOGITS_MAX_BIASES || a->vocab > (1 << 30))
+    return fail(-1, "process_logits: sequences, history, biases or vocabulary above their limits");
   if (a->rows == 0 || a->vocab == 0) return 0;
   if (!a->logits || !a->out || (a->history && !a->history_lens) || (a->num_biases && (!a->bias_ids || !a->bias_values)) ||
       (a->draft_tokens && !a->q_start))

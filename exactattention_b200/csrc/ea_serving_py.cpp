@@ -323,8 +323,10 @@ PyObject* process_logits(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
         need(t.dim() >= 1 && (batch < 0 || t.size(0) == batch), "the sequences' tensors differ in length");
         batch = t.size(0);
       }
-    if (batch < 0) batch = v[13] == Py_None ? rows : tensor(v[13], "q_start").numel() - 1;
+    // Where nothing says how many sequences there are, masks alone are left to apply: any row_seq may be one.
+    if (batch < 0) batch = v[13] != Py_None ? tensor(v[13], "q_start").numel() - 1 : v[1] == Py_None ? rows : EA_LOGITS_MAX_SEQS;
     need(v[1] != Py_None || batch == rows, "without row_seq there must be one row a sequence");
+    need(batch >= 0 && batch <= EA_LOGITS_MAX_SEQS, "process_logits: more sequences than its limit");
     ea_process_logits_t a = {};
     a.row_seq = ints(v[1], "row_seq", dev, rows);
     if (v[2] != Py_None) {

@@ -147,7 +147,9 @@ def process_logits(logits, row_seq=None, *, history=None, history_lens=None, pro
                    frequency=None, presence=None, bias_ids=None, bias_values=None, allowed_bits=None, mask_rows=None,
                    draft_tokens=None, q_start=None, tree_mask=None, out=None):
     """Penalties, biases and grammar masks (ea_process_logits_cuda) on logits (rows, vocab) of bf16, fp16 or
-    fp32; row r belongs to sequence row_seq[r] (int32; None: r; outside the batch: the row is copied).
+    fp32; row r belongs to sequence row_seq[r] (int32; None: r; outside the batch: the row is copied, its mask too
+    left out). The batch is the length of the sequences' tensors (history, repetition, frequency, presence, bias_ids, else
+    q_start); with masks alone every row_seq from 0 to 2^30 - 1 is a sequence.
     history (batch, width) int32 holds each sequence's tokens, the first prompt_lens[b] of its
     history_lens[b] being the prompt; draft_tokens (rows,) int32 with q_start (batch + 1,) and tree_mask (as
     for tree_attention; None: a chain) add the drafted tokens on each row's path. Then, in 32 bits and

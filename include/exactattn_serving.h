@@ -134,12 +134,13 @@ int ea_tree_attention_cuda(const ea_tree_attention_t* args, void* stream);
  *       0 .. num_masks - 1 allows every token)
  * rounded once to the type of logits. NULL history / repetition / frequency / presence / biases /
  * allowed_bits / draft_tokens leave their step out. Token ids outside 0 .. vocab - 1 are ignored;
- * rows with row_seq outside 0 .. batch - 1 are copied. out may be logits itself. At most
- * EA_LOGITS_MAX_HISTORY history entries, EA_LOGITS_MAX_PATH drafted tokens (later ones are not
- * counted) and EA_LOGITS_MAX_BIASES biases a sequence. */
+ * rows with row_seq outside 0 .. batch - 1 are copied, unmasked too. out may be logits itself. At most
+ * EA_LOGITS_MAX_SEQS sequences, EA_LOGITS_MAX_HISTORY history entries, EA_LOGITS_MAX_PATH drafted
+ * tokens (later ones are not counted) and EA_LOGITS_MAX_BIASES biases a sequence. */
 #define EA_LOGITS_MAX_HISTORY 1000000
 #define EA_LOGITS_MAX_PATH 32768
 #define EA_LOGITS_MAX_BIASES 2000
+#define EA_LOGITS_MAX_SEQS (1 << 30)
 typedef struct ea_process_logits {
   const void* logits; /* (rows, vocab), rows logits_stride elements apart */
   void* out;          /* (rows, vocab), rows out_stride apart */

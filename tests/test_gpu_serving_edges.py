@@ -161,3 +161,21 @@ def test_plan_step_page_counts_past_32_bits():
     assert p.slot_map.tolist() == [-1, 1, 2, -1, -1, -1, -1, -1] and p.token_seq.tolist() == [0, 1, 1, -1, -1, -1, -1, -1]
     assert p.q_start.tolist() == [0, 1, 3] and p.seq_lens.tolist() == [big, 2] and int(p.free_head) == 3
     assert table.tolist() == [[-1, -1, -1], [1, 2, -1]]
+
+
+@pytest.mark.parametrize("rows", [3, 1500])
+def test_process_logits_masks_alone_for_late_sequences(rows):
+    """Masks need no tensor of the sequences, so nothing says how many there are: the rows of a few late sequences of a
+    server (numbers above the row count) are masked like any others."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn((rows, 70), generator=g, device=DEV)
+    seqs = torch.arange(rows, device=DEV, dtype=torch.int32) * 7 + 5
+    seqs[1] = -1
+    states = torch.arange(rows, device=DEV, dtype=torch.int32) % 4
+    bits = torch.randint(-2**31, 2**31, (4, 3), generator=g, device=DEV).to(torch.int32)
+    bits[0] = 0
+    at = torch.arange(70, device=DEV)
+    allowed = ((bits[:, at // 32] >> (at % 32)) & 1).bool()[states.long()]
+    allowed[1] = True
+    want = x.masked_fill(~allowed, -math.inf)
+    assert torch.equal(serving.process_logits(x, seqs, allowed_bits=bits, mask_rows=states), want)
