@@ -66,7 +66,7 @@ int ea_plan_step_cuda(const ea_plan_step_t* args, void* stream);
  * slot_map[t] of k_cache and v copied to that row of v_cache (nothing is written at -1): slot s is
  * row s % page_size of page s / page_size, strides in elements. v and the caches are NULL without
  * slot_map. q (or k and v) may be NULL with its head count 0. Outputs may not overlap inputs.
- * d at most 1024. Angles keep 32-bit accuracy at positions of any size. */
+ * d at most 1024. Angles keep 32-bit accuracy at positions of any size and frequencies up to 2^40. */
 typedef struct ea_rope {
   const void *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;                /* between tokens, in elements */

@@ -2,6 +2,7 @@
 that one of the kernels or its host side once got wrong."""
 
 import ctypes
+import fractions
 import math
 import threading
 
@@ -11,7 +12,7 @@ import torch
 
 import serving_ref as ref
 from exactattention_b200 import _lib, serving
-from test_gpu_serving import DEV, attention_inputs, check_attention, i32
+from test_gpu_serving import DEV, attention_inputs, check_attention, check_rope, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +180,33 @@ def test_process_logits_masks_alone_for_late_sequences(rows):
     allowed[1] = True
     want = x.masked_fill(~allowed, -math.inf)
     assert torch.equal(serving.process_logits(x, seqs, allowed_bits=bits, mask_rows=states), want)
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("top", [0.5, 50.0, 1000.0, 3e4])
+def test_rope_large_angles(top, inverse):
+    """Positions below 2^24 with frequencies above 1, whose products lie far past 2^24, and the ends of the positions'
+    range. Their products are exact in binary64, up to the last two bits of the largest ones."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    n, d = 200, 64
+    q = torch.randn((n, 2, d), generator=g, device=DEV)
+    pos = torch.randint(0, 2**24, (n,), generator=g, device=DEV, dtype=torch.int32)
+    freq = top * torch.rand(d // 2, generator=g, device=DEV) + top / 50
+    if top < 1:
+        pos[:4] = torch.tensor([-2**31, 2**31 - 1, -2**24, 2**24], device=DEV)
+    check_rope(serving.rope(q, None, pos, freq, inverse=inverse)[0], q, pos, freq, None, "half", inverse)
+
+
+def test_rope_huge_angles():
+    """Angles up to 2^71, reduced for the comparison with 1 / (2 pi) to 192 bits."""
+    inv_2pi = fractions.Fraction(0x28BE60DB9391054A7F09D5F47D4D377036D8A5664F10E410, 2**192)  # 1 / (2 pi) to 2^-192
+    pos = [1, 3, 12345677, 2**31 - 1, -2**31, 2**24 + 1]
+    f0 = torch.tensor([1.0, 1.25, 0.7853982, 0.001], dtype=torch.float32)
+    q = torch.zeros((len(pos), 1, 8), device=DEV)
+    q[..., :4] = 1  # the result is (cos, sin)
+    got = serving.rope(q, None, i32(pos), (2.0**40 * f0).to(DEV))[0].cpu().double()
+    for t, p in enumerate(pos):
+        for i, f in enumerate(f0.tolist()):
+            turns = p * fractions.Fraction(f) * 2**40 * inv_2pi
+            a = 2 * math.pi * float(turns - round(turns))
+            assert abs(float(got[t, 0, i]) - math.cos(a)) <= 2.0**-20 and abs(float(got[t, 0, 4 + i]) - math.sin(a)) <= 2.0**-20
