@@ -529,8 +529,11 @@ extern "C" int ea_tree_attention_cuda(const ea_tree_attention_t* t, void* stream
       (t->max_pages && (!t->page_table || !t->k_cache || !t->v_cache)))
     return fail(-1, "tree_attention: a required pointer is NULL");
   const uintptr_t base = (uintptr_t)t->q | (uintptr_t)t->k_cache | (uintptr_t)t->v_cache | (uintptr_t)t->out | (uintptr_t)t->workspace;
-  const int64_t strides = t->q_stride | t->q_head_stride | t->k_page_stride | t->k_head_stride | t->k_row_stride |
-                          t->v_page_stride | t->v_head_stride | t->v_row_stride;
+  const auto used = [](int64_t extent, int64_t stride, int64_t other) { return extent > 1 ? stride | other : 0; };
+  const int64_t strides = used(t->tokens, t->q_stride, 0) | used(t->q_heads, t->q_head_stride, 0) |
+                          used(t->num_pages, t->k_page_stride, t->v_page_stride) |
+                          used(t->kv_heads, t->k_head_stride, t->v_head_stride) |
+                          used(t->page_size, t->k_row_stride, t->v_row_stride);
   if (base % 16 || strides % 8) return fail(-9, "tree_attention: rows of q, the caches or out, or the workspace, are not on 16-byte boundaries");
   tree::Args a;
   a.t = *t;

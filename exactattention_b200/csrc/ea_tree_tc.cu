@@ -33,12 +33,13 @@ bool tensor_map(const Args& a, bool value, int box, CUtensorMap* tm) {
   memset(tm, 0, sizeof *tm);
   const int64_t strides[3] = {value ? a.t.v_row_stride : a.t.k_row_stride, value ? a.t.v_head_stride : a.t.k_head_stride,
                               value ? a.t.v_page_stride : a.t.k_page_stride};
+  const cuuint64_t dims[4] = {(cuuint64_t)a.t.d, (cuuint64_t)a.t.page_size, (cuuint64_t)a.t.kv_heads, (cuuint64_t)a.t.num_pages};
   cuuint64_t bytes[3];
   for (int i = 0; i < 3; ++i) {
-    if (strides[i] <= 0 || strides[i] >= (1ll << 38)) return false;
-    bytes[i] = (cuuint64_t)strides[i] * 2;
+    const int64_t stride = dims[i + 1] > 1 ? strides[i] : a.t.d;  // of an extent of one it may be anything, but not in the map
+    if (stride <= 0 || stride >= (1ll << 38)) return false;
+    bytes[i] = (cuuint64_t)stride * 2;
   }
-  const cuuint64_t dims[4] = {(cuuint64_t)a.t.d, (cuuint64_t)a.t.page_size, (cuuint64_t)a.t.kv_heads, (cuuint64_t)a.t.num_pages};
   const cuuint32_t tile[4] = {64u, (cuuint32_t)box, 1u, 1u}, step[4] = {1u, 1u, 1u, 1u};
   return encode && a.t.num_pages > 0 && a.t.num_pages < (1ll << 31) &&
          encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, (void*)(value ? a.t.v_cache : a.t.k_cache), dims, bytes, tile, step,

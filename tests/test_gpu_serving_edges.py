@@ -210,3 +210,22 @@ def test_rope_huge_angles():
             turns = p * fractions.Fraction(f) * 2**40 * inv_2pi
             a = 2 * math.pi * float(turns - round(turns))
             assert abs(float(got[t, 0, i]) - math.cos(a)) <= 2.0**-20 and abs(float(got[t, 0, 4 + i]) - math.sin(a)) <= 2.0**-20
+
+
+@pytest.mark.parametrize("new,pages", [(1, 1), (1, 7), (40, 1), (40, 9)])
+def test_tree_attention_strides_of_extents_of_one(new, pages):
+    """A stride over an extent of one says nothing: one token, one kv head or one page of a buffer of odd rows."""
+    ps = 64 if pages == 1 else 16
+    x = attention_inputs([min(ps * pages, 130) - new - 3], [new], 4, 1, 64, ps, torch.bfloat16)
+    if pages == 1:
+        page = int(x["page_table"][0, 0])
+        x.update(k_cache=x["k_cache"][page:page + 1], v_cache=x["v_cache"][page:page + 1], page_table=i32([[0]]))
+    want = serving.tree_attention(**x)
+
+    def odd(t):
+        strides = [n if size > 1 else 7777777 for n, size in zip(t.stride(), t.shape)]
+        return torch.as_strided(t, t.shape, strides, t.storage_offset())
+
+    y = dict(x, q=odd(x["q"]), k_cache=odd(x["k_cache"]), v_cache=odd(x["v_cache"]))
+    assert any(s % 8 for s in y["k_cache"].stride())
+    assert torch.equal(serving.tree_attention(**y), want)
