@@ -5,6 +5,7 @@
 // GPU; this module's calls cost 3-6 us. serving.py holds the documented functions, which pass their
 // arguments on by position. Wrong arguments raise ValueError, tensors off the GPU and CUDA errors RuntimeError.
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -25,7 +26,11 @@ void need(bool ok, const char* msg) {
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) throw Refused(std::string(name) + " must be a tensor");
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  // the operators record no graph: a gradient through them would be dropped without a word
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    throw Refused(std::string(name) + " requires grad, which the serving operators do not record (torch.no_grad, or detach it)");
+  return t;
 }
 
 int64_t integer(PyObject* o, const char* name) {

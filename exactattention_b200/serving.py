@@ -10,7 +10,9 @@ positions, the draft model's attention over the paged cache, and the logits' pen
 Ordinary floating-point operators (32-bit arithmetic, outputs rounded once), hand-written CUDA behind
 include/exactattn_serving.h. Drafts are proposals: the bits that count come from the certified
 `cuda.launch`, which verifies them over the same cache. Torch CUDA tensors in and out, asynchronous on
-the current stream, no host synchronisation, capturable in CUDA graphs. There is no CPU path.
+the current stream, no host synchronisation, capturable in CUDA graphs. There is no CPU path. Nothing is
+recorded for autograd: tensors that require grad are refused (ValueError) unless under torch.no_grad; a
+training loop calls rope and its `inverse` from a torch.autograd.Function of its own.
 """
 
 from __future__ import annotations

@@ -229,3 +229,25 @@ def test_tree_attention_strides_of_extents_of_one(new, pages):
     y = dict(x, q=odd(x["q"]), k_cache=odd(x["k_cache"]), v_cache=odd(x["v_cache"]))
     assert any(s % 8 for s in y["k_cache"].stride())
     assert torch.equal(serving.tree_attention(**y), want)
+
+
+def test_rope_in_a_training_step():
+    """rope and its inverse as the two directions of an autograd function; called bare, it refuses what requires grad."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q = torch.randn((9, 4, 64), generator=g, device=DEV, requires_grad=True)
+    dy = torch.randn((9, 4, 64), generator=g, device=DEV)
+    pos, freq = i32(np.arange(9) * 100), 1e4 ** (-torch.arange(0, 64, 2, device=DEV) / 64)
+
+    class Rope(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return serving.rope(x, None, pos, freq)[0]
+
+        @staticmethod
+        def backward(ctx, d):
+            return serving.rope(d, None, pos, freq, inverse=True)[0]
+
+    with pytest.raises(ValueError, match="requires grad"):
+        serving.rope(q, None, pos, freq)
+    Rope.apply(q).backward(dy)
+    check_rope(q.grad, dy, pos, freq, None, "half", True)

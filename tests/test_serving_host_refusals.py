@@ -3,8 +3,9 @@
 import ctypes
 
 import pytest
+import torch
 
-from exactattention_b200 import _lib
+from exactattention_b200 import _lib, serving
 
 
 @pytest.mark.parametrize("off", [2, 4, 8, 24])
@@ -22,3 +23,23 @@ def test_tree_attention_refuses_rows_off_16_byte_boundaries(cuda_lib, name, off)
     setattr(t, name, getattr(t, name) + off)
     assert cuda_lib.ea_tree_attention_cuda(ctypes.byref(t), None) == -9
     assert b"16-byte" in cuda_lib.ea_serving_last_error()
+
+
+@pytest.mark.parametrize("call", [
+    lambda x: serving.rope(x, None, torch.zeros(3, dtype=torch.int32), torch.zeros(32)),
+    lambda x: serving.rope(torch.zeros(3, 2, 64), x, torch.zeros(3, dtype=torch.int32), torch.zeros(32)),
+    lambda x: serving.rope(torch.zeros(3, 2, 64), None, torch.zeros(3, dtype=torch.int32), x[0, 0, :32]),
+    lambda x: serving.tree_attention(x, torch.zeros(5, 2, 16, 64), torch.zeros(5, 2, 16, 64), torch.zeros(2, 4, dtype=torch.int32),
+                                     torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), 0.1),
+    lambda x: serving.process_logits(x[0]),
+])
+def test_tensors_that_require_grad_are_refused(cuda_lib, call):
+    """No graph is recorded, so a gradient would be lost silently; without grad mode there is none to lose."""
+    x = torch.zeros(3, 2, 64, requires_grad=True)
+    with pytest.raises(ValueError, match="requires grad"):
+        call(x)
+    with torch.no_grad():
+        try:
+            call(x)
+        except (RuntimeError, ValueError) as e:  # CPU tensors, or a type that the operator does not take
+            assert "requires grad" not in str(e)
