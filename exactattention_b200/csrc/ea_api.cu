@@ -1060,6 +1060,13 @@ extern "C" int ea_set_test_hooks(const ea_test_hooks_t* h) {
   return 0;
 }
 
+// For the serving operators' launches, which have no problem description.
+namespace ea {
+namespace serving {
+int wait_debug_hook() { return g_hooks.wait_debug; }
+}  // namespace serving
+}  // namespace ea
+
 // Diagnostic: device time of the tier-1 kernel of each ea_launch_cuda call (the hot kernel:
 // tensor-core prefill / decode, or the CUDA-core split kernel with its combine).
 extern "C" int ea_kernel_timing(int mode, double* total_ms, int64_t* launches) {

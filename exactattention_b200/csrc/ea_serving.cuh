@@ -15,6 +15,8 @@ namespace serving {
 int fail(int code, const char* msg);
 // 0, or -4 with the CUDA error's text.
 int cuda_rc(cudaError_t e);
+// wait_debug of ea_set_test_hooks (ea_api.cu).
+int wait_debug_hook();
 // SMs of the current device (looked up once per device).
 int sm_count();
 

@@ -541,6 +541,7 @@ extern "C" int ea_tree_attention_cuda(const ea_tree_attention_t* t, void* stream
   a.by_page = fast_div((uint32_t)t->page_size);
   a.by_group = fast_div((uint32_t)a.group);
   a.dp = t->d <= 64 ? 64 : 128;
+  a.wait_debug = wait_debug_hook();
   const tree::Choice c = tree::choose(*t);
   a.workers = tree::workers_for(*t, c);
   cudaStream_t st = (cudaStream_t)stream;

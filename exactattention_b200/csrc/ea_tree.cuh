@@ -21,6 +21,7 @@ struct Args {
   int group;     // query heads per kv head
   int workers;   // blocks that share the units
   int dp;        // channels of a partial: d rounded up
+  int wait_debug;  // test hook (ea_set_test_hooks): the bounded waits report expiry
 };
 
 // The reference m of a row's weights 2^(s - m), in powers of two. When it moves it is put DOWN below the largest score seen;

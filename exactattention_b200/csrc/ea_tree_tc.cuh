@@ -99,8 +99,9 @@ __device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
       "r"(leader)
       : "memory");
 }
-// Bounded wait that reads the timer only when the phase is late (a read costs some 300 cycles).
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
+// Bounded wait that reads the timer only when the phase is late (a read costs some 300 cycles). `debug` (the test hook): the limit
+// is 20 ms instead of 2 s. (Asking for it before the loop, at every wait, cost 5 to 11% of a call.)
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int debug) {
   const uint32_t a = smem_u32(bar);
 #pragma unroll 1
   for (int i = 0; i < 256; ++i) {
@@ -112,7 +113,7 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
         : "memory");
     if (done) return true;
   }
-  return mbar_wait(bar, parity);
+  return mbar_wait(bar, parity, debug);
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Item it = sch.item(a, pos, end);
       pos = it.next;
       if (it.kt0 >= it.kt1) continue;
-      if (items) alive = __all_sync(0xffffffffu, wait_phase(&sh.q_free, (items - 1) & 1));
+      if (items) alive = __all_sync(0xffffffffu, wait_phase(&sh.q_free, (items - 1) & 1, a.wait_debug));
       if (!alive) break;
       ++items;
       constexpr int PIECES = DP / 8;
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int i = 0; i < 4; ++i) w[i] = a.t.alpha < 0 ? w[i] ^ 0x80008000u : 0u;
         }
       fence_async_smem();
-      arrive(&sh.q_full);
+      if (!a.wait_debug) arrive(&sh.q_full);  // with the hook what waits for this, and all that waits for that, runs out
     }
   } else if (warp >= 9 && box) {
     // ---- loader warp, tensor copies: a lane issues one box (64 channels x `box` rows of one page) of every tile
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         };
         const auto load = [&](int t, int page, bool value) {
           const uint32_t b = cnt % NBUF;
-          if (cnt >= NBUF) alive = __all_sync(0xffffffffu, wait_phase(&sh.empty[b], (cnt / NBUF - 1) & 1));
+          if (cnt >= NBUF) alive = __all_sync(0xffffffffu, wait_phase(&sh.empty[b], (cnt / NBUF - 1) & 1, a.wait_debug));
           if (!alive) return;
           if (!value) {  // which of the tile's keys have a page
             const uint32_t bits = page < 0 ? 0u : box >= 32 ? 0xFFFFFFFFu : ((1u << box) - 1) << (sub * box & 31);
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (cnt >= NBUF) {
           const uint32_t parity = (cnt / NBUF - 1) & 1;
           while (pending && !__all_sync(0xffffffffu, try_now(&sh.empty[b], parity))) retire();
-          alive = __all_sync(0xffffffffu, wait_phase(&sh.empty[b], parity));
+          alive = __all_sync(0xffffffffu, wait_phase(&sh.empty[b], parity, a.wait_debug));
           if (!alive) return;
         }
         if (pending == 7) retire();
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t cnt = 0, items = 0, phases = 0;  // tiles taken from the ring; items; bit s: parity of slot s's weights
       const uint32_t qd = desc_lo(smem_u32(qbuf), 16), ring_at = smem_u32(ring);
       const auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (alive) alive = __all_sync(0xffffffffu, wait_phase(bar, parity));
+        if (alive) alive = __all_sync(0xffffffffu, wait_phase(bar, parity, a.wait_debug));
       };
       while (pos < end && alive) {
         const Item it = sch.item(a, pos, end);
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const float scale_s = a.t.alpha == 0 ? 1.0f : fabsf(a.t.alpha);
     uint32_t ns = 0, first = 0, items = 0;  // phases of s_full seen; ring position of the item's first tile; items
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (alive) alive = __all_sync(0xffffffffu, wait_phase(bar, parity));
+      if (alive) alive = __all_sync(0xffffffffu, wait_phase(bar, parity, a.wait_debug));
     };
     while (pos < end) {
       const Item it = sch.item(a, pos, end);

@@ -303,8 +303,9 @@ int ea_last_host_stats(int64_t* out);
  * bits must not change. wait_debug != 0: every bounded wait of the tensor-core kernels reports
  * expiry once its phase has completed (or after 20 ms), so their abort path runs with nothing left
  * in flight: stats[8] counts the CTAs, their rows are recomputed by the later tiers, and the
- * host-pointer entry points return -5. Applies to every device, to launches made after the call;
- * NULL resets. Returns 0 or -1. No reference counterpart as an entry point: the reference drives
+ * host-pointer entry points return -5. In ea_tree_attention_cuda (exactattn_serving.h) the waits of
+ * the tensor-core kernel run out after 20 ms, and its rows come back as NaN. Applies to every device,
+ * to launches made after the call; NULL resets. Returns 0 or -1. No reference counterpart as an entry point: the reference drives
  * its fallback tiers in tests by narrowing its windows (Config(acc_bits=34),
  * tests/test_certified.py:129-139). */
 typedef struct ea_test_hooks {

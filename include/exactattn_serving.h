@@ -100,7 +100,9 @@ int ea_rope_cuda(const ea_rope_t* args, void* stream);
  * workspace: ea_tree_attention_workspace(args) bytes, 16-byte aligned, any contents; calls that
  * may overlap need workspaces of their own. Page ids outside 0 .. num_pages - 1 and keys past the table's
  * columns are read as keys no row sees; tokens past `tokens` have no row, but still count among the step's.
- * Deterministic for equal inputs on one GPU model (no atomics). */
+ * Deterministic for equal inputs on one GPU model (no atomics).
+ * Waits inside the kernels are bounded (2 s): rows whose block gave one up are NaN in out and lse, so that an error
+ * shows in the results; it has never been seen outside of the test hook (ea_set_test_hooks). */
 #define EA_TREE_MAX_SEQS 8192
 typedef struct ea_tree_attention {
   const void* q; /* (tokens, q_heads, d) */

@@ -251,3 +251,20 @@ def test_rope_in_a_training_step():
         serving.rope(q, None, pos, freq)
     Rope.apply(q).backward(dy)
     check_rope(q.grad, dy, pos, freq, None, "half", True)
+
+
+@pytest.mark.parametrize("new,hq,ps", [(40, 4, 16), (40, 4, 24), (300, 4, 16), (300, 4, 24)])
+def test_tree_attention_waits_that_run_out(new, hq, ps):
+    """With the hook the tensor-core kernel's queries are never announced, so its products, copies and softmax wait in vain
+    for 20 ms: the rows come back as NaN, what was under way has landed, and the next call is right."""
+    x = attention_inputs([500, 90, 3000], [new, 3, 20], hq, 1, 64, ps, torch.bfloat16)
+    want = serving.tree_attention(**x, return_lse=True)
+    try:
+        _lib.set_test_hooks(0, 0, 1)
+        out, lse = serving.tree_attention(**x, return_lse=True)
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_test_hooks(0, 0, 0)
+    assert bool(torch.isnan(out).all()) and bool(torch.isnan(lse).all())
+    for a, b in zip(serving.tree_attention(**x, return_lse=True), want):
+        assert torch.equal(a, b)
