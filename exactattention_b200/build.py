@@ -79,19 +79,31 @@ def build_synth_host(force: bool = False) -> str:
 SERVING_NATIVE = os.path.join(HERE, "_serving_native" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
+def _serving_native_current(so: str) -> bool:
+    """Whether the binding is newer than its sources and was built against the torch that is installed: its ABI is
+    torch's C++ ABI, which changes from version to version. The version is in the module's `torch_version` string."""
+    deps = [os.path.join(CSRC, "ea_serving_py.cpp"), HEADERS[1]]
+    if not os.path.exists(so) or os.path.getmtime(so) < max(map(os.path.getmtime, deps)):
+        return False
+    import torch
+
+    with open(so, "rb") as f:
+        return f"built against torch {torch.__version__}\0".encode() in f.read()
+
+
 def build_serving_native(force: bool = False) -> str:
     """The Python binding of the serving operators (csrc/ea_serving_py.cpp), g++ against torch's headers; it
     finds libexactattn_cuda.so beside itself."""
-    src = os.path.join(CSRC, "ea_serving_py.cpp")
-    deps = [src, HEADERS[1]]
-    if force or not os.path.exists(SERVING_NATIVE) or os.path.getmtime(SERVING_NATIVE) < max(map(os.path.getmtime, deps)):
+    if force or not _serving_native_current(SERVING_NATIVE):
+        import torch
         from torch.utils import cpp_extension
 
         cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))
         inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
         lib = cpp_extension.library_paths()
-        subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-I{p}" for p in inc], "-o", SERVING_NATIVE + ".tmp",
-                        src, *[f"-L{p}" for p in lib], f"-L{HERE}", "-l:libexactattn_cuda.so", "-lc10", "-lc10_cuda",
+        subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f'-DEA_TORCH_VERSION="{torch.__version__}"',
+                        *[f"-I{p}" for p in inc], "-o", SERVING_NATIVE + ".tmp", os.path.join(CSRC, "ea_serving_py.cpp"),
+                        *[f"-L{p}" for p in lib], f"-L{HERE}", "-l:libexactattn_cuda.so", "-lc10", "-lc10_cuda",
                         "-ltorch_cpu",
                         "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], check=True)
         os.replace(SERVING_NATIVE + ".tmp", SERVING_NATIVE)

@@ -390,4 +390,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving_native", nullptr, -1, met
 
 }  // namespace
 
-extern "C" PyObject* PyInit__serving_native() { return PyModule_Create(&module); }
+extern "C" PyObject* PyInit__serving_native() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", "built against torch " EA_TORCH_VERSION) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -47,6 +47,10 @@ def _native():
             from . import _serving_native
         except ImportError as e:
             raise RuntimeError(f"{e}: build it with `python -m exactattention_b200.build`") from e
+        built = getattr(_serving_native, "torch_version", "built against another torch")
+        if built != f"built against torch {torch.__version__}":
+            raise RuntimeError(f"{_serving_native.__file__} was {built}, this is {torch.__version__}: "
+                               "build it with `python -m exactattention_b200.build`")
         _mod = _serving_native
     return _mod
 

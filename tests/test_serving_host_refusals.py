@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from exactattention_b200 import _lib, serving
+from exactattention_b200 import _lib, build, serving
 
 
 @pytest.mark.parametrize("off", [2, 4, 8, 24])
@@ -43,3 +43,13 @@ def test_tensors_that_require_grad_are_refused(cuda_lib, call):
             call(x)
         except (RuntimeError, ValueError) as e:  # CPU tensors, or a type that the operator does not take
             assert "requires grad" not in str(e)
+
+
+def test_a_binding_of_another_torch_is_not_used(cuda_lib, monkeypatch):
+    """The binding uses torch's C++ ABI: after a change of torch it counts as stale, and is refused until it is rebuilt."""
+    assert build._serving_native_current(build.SERVING_NATIVE)
+    monkeypatch.setattr(torch, "__version__", "2.99.0")
+    assert not build._serving_native_current(build.SERVING_NATIVE)
+    monkeypatch.setattr(serving, "_mod", None)
+    with pytest.raises(RuntimeError, match="this is 2.99.0"):
+        serving._native()
