@@ -268,3 +268,43 @@ def test_tree_attention_waits_that_run_out(new, hq, ps):
     assert bool(torch.isnan(out).all()) and bool(torch.isnan(lse).all())
     for a, b in zip(serving.tree_attention(**x, return_lse=True), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq", [2, 7, 8, 16])
+def test_tree_attention_few_rows_carry_weights_as_pairs(dtype, hq):
+    """Up to 16 rows a kv head take a weight as two 16-bit numbers, 2^-17 off in all. Pairs of keys with almost the same score and
+    opposite values leave next to nothing but the weights' errors: a single 16-bit rounding is 4 to 20 times the bound."""
+    n, d = 80, 8
+    x = attention_inputs([n - 1] * 6, [1] * 6, hq, 1, d, 16, dtype, mask="chain")
+    g = torch.Generator(device=DEV).manual_seed(hq)
+    low = torch.randn((6, n // 2), generator=g, device=DEV).to(dtype)
+    up = (low.float() * (1 + 2.0**-7 if dtype == torch.bfloat16 else 1 + 2.0**-10)).to(dtype)
+    score = torch.stack([low, up], -1).reshape(6, n)
+    x["q"].zero_(), x["k_cache"].zero_()
+    x["q"][..., 0] = 1
+    for b in range(6):
+        key = torch.arange(n, device=DEV)
+        page = x["page_table"][b].long()[key // 16]
+        x["k_cache"][page, 0, key % 16, 0] = score[b]
+        x["v_cache"][page, 0, key % 16] = (1.0 - 2.0 * (key % 2))[:, None].to(dtype)
+    out = serving.tree_attention(**dict(x, alpha=1.0), max_new=1).double()
+    w, sign = torch.exp2(score.double()), 1.0 - 2.0 * (torch.arange(n, device=DEV) % 2)
+    o = (w * sign).sum(1) / w.sum(1)
+    # scores of d terms in 32 bits, a weight's pair, exp2 and the sums of at most 16 steps
+    rel = 2 * math.log(2) * d * 2.0**-23 * score.double().abs().amax(1) + 2.0**-17 + 2.0**-18
+    bound = ref.HALF_ULP[dtype] * o.abs() + rel + ref.TINY[dtype]
+    ref.assert_within(out, o[:, None, None].expand_as(out), bound[:, None, None].expand_as(out))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,limit", [(1, 1.05), (8, 1.05), (40, 1.6), (300, 1.6)])
+def test_tree_attention_error_over_a_long_context(dtype, new, limit):
+    """The root mean square error against the output's own rounding: the same for up to 16 rows a kv head, whose weights'
+    errors do not show; up to 2^(1/2) times it (and a tenth for the sample) on the tensor cores, where a weight's
+    rounding is one of the same size and sign."""
+    x = attention_inputs([3000], [new], 8, 4, 128, 16, dtype)
+    o, _, _, _ = reference(x)
+    out = serving.tree_attention(**x, max_new=new).double()
+    rms = lambda e: float(e.square().mean().sqrt())  # noqa: E731
+    assert rms(out - o) <= limit * rms(o.to(dtype).double() - o)
