@@ -93,9 +93,14 @@ def _serving_native_current(so: str) -> bool:
 
 def build_serving_native(force: bool = False) -> str:
     """The Python binding of the serving operators (csrc/ea_serving_py.cpp), g++ against torch's headers; it
-    finds libexactattn_cuda.so beside itself."""
-    if force or not _serving_native_current(SERVING_NATIVE):
+    finds libexactattn_cuda.so beside itself. Without torch, which the rest of the package needs only for torch
+    tensors, it is left out."""
+    try:
         import torch
+    except ImportError:
+        print("no torch: the Python binding of the serving operators is not built", file=sys.stderr)
+        return SERVING_NATIVE
+    if force or not _serving_native_current(SERVING_NATIVE):
         from torch.utils import cpp_extension
 
         cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))

@@ -1,6 +1,9 @@
 """What the serving operators refuse on the host, before any launch, beyond test_serving_host.py."""
 
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -53,3 +56,14 @@ def test_a_binding_of_another_torch_is_not_used(cuda_lib, monkeypatch):
     monkeypatch.setattr(serving, "_mod", None)
     with pytest.raises(RuntimeError, match="this is 2.99.0"):
         serving._native()
+
+
+def test_the_library_builds_without_torch(cuda_lib):
+    """The certified entry points take numpy arrays and need no torch, and neither does their build."""
+    code = ("import sys; sys.modules['torch'] = None\n"
+            "import exactattention_b200\nfrom exactattention_b200 import _lib, build\n"
+            "assert build.build() == build.OUT and _lib.load()\n")
+    root = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0, run.stderr[-2000:]
+    assert "no torch" in run.stderr
