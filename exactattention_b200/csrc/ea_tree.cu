@@ -476,20 +476,6 @@ int64_t most_units(const ea_tree_attention_t& t, int rows, int kt) {
   return row_tiles * t.kv_heads * ((tiles > 0 ? tiles : 1) + 4);  // and an item's units without keys
 }
 
-int check(const ea_tree_attention_t* t) {
-  if (!t || t->tokens < 0 || t->batch < 0 || t->q_heads <= 0 || t->kv_heads <= 0 || t->d <= 0 || t->page_size <= 0 ||
-      t->max_pages < 0 || t->num_pages < 0 || t->mask_words < 0)
-    return fail(-1, "tree_attention: negative or zero size");
-  if (t->q_heads % t->kv_heads) return fail(-1, "tree_attention: q_heads is no multiple of kv_heads");
-  if (t->batch > EA_TREE_MAX_SEQS) return fail(-1, "tree_attention: more than EA_TREE_MAX_SEQS sequences");
-  if (t->d % 8 || t->d > 128) return fail(-9, "tree_attention: d is no multiple of 8 up to 128");
-  if (t->dtype != EA_BF16 && t->dtype != EA_FP16) return fail(-9, "tree_attention: element type is neither bf16 nor fp16");
-  if (t->tokens * t->q_heads >= (1ll << 31) || (int64_t)t->max_pages * t->page_size >= (1ll << 31) ||
-      most_units(*t, 8, KT) >= (1ll << 31))
-    return fail(-1, "tree_attention: too many tokens or keys");
-  return 0;
-}
-
 // Which kernel, by the query rows per sequence and kv head: at most 8 or 16 (few_rows_kernel), below 512 the tensor-core
 // kernel with 128-row items, else with 256-row items, which take half the traffic from L2 but keep one of two slots
 // idle where an item has 128 rows or fewer (2048 rows: 345 us against 370 us; 7 to 231 rows: 73 us against 68 us).
@@ -502,6 +488,22 @@ Choice choose(const ea_tree_attention_t& t) {
   if (rows <= MAX_ROWS || t.batch > MANY_MAX_SEQS) return {rows <= 8 ? 8 : MAX_ROWS, KT, 2};
   return {rows < 512 ? 128 : 256, 128, 1};
 }
+int check(const ea_tree_attention_t* t) {
+  if (!t || t->tokens < 0 || t->batch < 0 || t->q_heads <= 0 || t->kv_heads <= 0 || t->d <= 0 || t->page_size <= 0 ||
+      t->max_pages < 0 || t->num_pages < 0 || t->mask_words < 0)
+    return fail(-1, "tree_attention: negative or zero size");
+  if (t->q_heads % t->kv_heads) return fail(-1, "tree_attention: q_heads is no multiple of kv_heads");
+  if (t->batch > EA_TREE_MAX_SEQS) return fail(-1, "tree_attention: more than EA_TREE_MAX_SEQS sequences");
+  if (t->d % 8 || t->d > 128) return fail(-9, "tree_attention: d is no multiple of 8 up to 128");
+  if (t->dtype != EA_BF16 && t->dtype != EA_FP16) return fail(-9, "tree_attention: element type is neither bf16 nor fp16");
+  if (t->tokens * t->q_heads >= (1ll << 31) || (int64_t)t->max_pages * t->page_size >= (1ll << 31))
+    return fail(-1, "tree_attention: too many tokens or keys");
+  const Choice c = choose(*t);
+  if (most_units(*t, c.rows, c.kt) >= (1ll << 31))
+    return fail(-1, "tree_attention: 2^31 tiles or more, by the tokens, the table's width and max_new");
+  return 0;
+}
+
 int workers_for(const ea_tree_attention_t& t, const Choice& c) {
   const int64_t most = most_units(t, c.rows, c.kt), fill = (int64_t)c.per_sm * sm_count();
   return (int)(most < fill ? (most > 0 ? most : 1) : fill);

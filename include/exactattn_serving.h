@@ -96,7 +96,8 @@ int ea_rope_cuda(const ea_rope_t* args, void* stream);
  * What a row does not see cannot reach its output, NaN and infinities included.
  * bf16 or fp16 (q, caches and out alike), d a multiple of 8 up to 128, rows on 16-byte boundaries (-9
  * otherwise).
- * max_new: the most tokens any sequence has in this step (a hint: it sizes tiles, not results).
+ * max_new: the most tokens any sequence has in this step (a hint: it sizes tiles, not results). tokens *
+ * q_heads, max_pages * page_size and the tiles that these allow stay below 2^31 (-1 otherwise).
  * workspace: ea_tree_attention_workspace(args) bytes, 16-byte aligned, any contents; calls that
  * may overlap need workspaces of their own. Page ids outside 0 .. num_pages - 1 and keys past the table's
  * columns are read as keys no row sees; tokens past `tokens` have no row, but still count among the step's.

@@ -308,3 +308,14 @@ def test_tree_attention_error_over_a_long_context(dtype, new, limit):
     out = serving.tree_attention(**x, max_new=new).double()
     rms = lambda e: float(e.square().mean().sqrt())  # noqa: E731
     assert rms(out - o) <= limit * rms(o.to(dtype).double() - o)
+
+
+def test_tree_attention_padded_step_over_a_wide_table():
+    """Rows for 32768 tokens and a table for a million keys, of which a step uses 300 and 800."""
+    x = attention_inputs([500], [300], 64, 8, 64, 16, torch.bfloat16, mask="chain")
+    want = serving.tree_attention(**x, max_new=300)
+    q = torch.zeros((32768, 64, 64), dtype=torch.bfloat16, device=DEV)
+    q[:300] = x["q"]
+    table = torch.full((1, 65536), -1, dtype=torch.int32, device=DEV)
+    table[:, :x["page_table"].shape[1]] = x["page_table"]
+    assert torch.equal(serving.tree_attention(**dict(x, q=q, page_table=table), max_new=300)[:300], want)

@@ -28,6 +28,18 @@ def test_tree_attention_refuses_rows_off_16_byte_boundaries(cuda_lib, name, off)
     assert b"16-byte" in cuda_lib.ea_serving_last_error()
 
 
+def test_tree_attention_counts_the_tiles_of_the_kernel_it_takes(cuda_lib):
+    """A prompt's chunk over a table wide enough for a million keys is 2^32 tiles of 8 rows x 64 keys, of which the kernel for
+    few rows would have more than it can count, but 2^26 of the ones that it runs in."""
+    t = _lib.TreeAttentionArgs()
+    t.tokens, t.batch, t.q_heads, t.kv_heads, t.d, t.page_size, t.max_pages, t.num_pages = 32768, 1, 64, 8, 128, 16, 65536, 4
+    t.max_new = 32768
+    assert cuda_lib.ea_tree_attention_workspace(ctypes.byref(t)) >= 0
+    t.max_new = 1
+    assert cuda_lib.ea_tree_attention_workspace(ctypes.byref(t)) == -1
+    assert b"2^31 tiles" in cuda_lib.ea_serving_last_error()
+
+
 @pytest.mark.parametrize("call", [
     lambda x: serving.rope(x, None, torch.zeros(3, dtype=torch.int32), torch.zeros(32)),
     lambda x: serving.rope(torch.zeros(3, 2, 64), x, torch.zeros(3, dtype=torch.int32), torch.zeros(32)),
