@@ -77,6 +77,8 @@ class KvAppendArgs(ctypes.Structure):
                 ("d", ctypes.c_int), ("advance_lens", ctypes.c_int)]
 
 
+# The argument structs of the serving entries, for callers through ctypes (the tests of the C entries; Python's own calls
+# go through csrc/ea_serving_py.cpp).
 def _fields(spec: str):
     """ctypes fields of "type: name name; ..." (p pointer, l int64, i int, f float)."""
     kinds = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float}

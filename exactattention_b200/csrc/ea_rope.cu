@@ -10,8 +10,8 @@
 // integer taken off the large part (exact); what is left of 2^-47 relative error is far below a 32-bit result's
 // rounding. sincospif then sees an argument in [-1, 1] whatever the position. Positions of 2^24 and more, which
 // binary32 does not hold, and angles of 2^24 and more, whose 2^-47 would show, are reduced the same way in binary64.
-// Measured on one B200: 16927 tokens, 16 q and 8 kv heads of 128, three axes, written into a paged cache: 54 us for 278 MB
-// (79% of the copy rate); with the angles computed per thread in binary64 127 us.
+// Measured on one B200: 16927 tokens, 16 q and 8 kv heads of 128, three axes, written into a paged cache: 53 us for 278 MB
+// (80% of the copy rate); with the angles computed per thread in binary64 127 us.
 #include "ea_serving.cuh"
 
 namespace ea {

@@ -478,8 +478,11 @@ int64_t most_units(const ea_tree_attention_t& t, int rows, int kt) {
 
 // Which kernel, by the query rows per sequence and kv head: at most 8 or 16 (few_rows_kernel), below 512 the tensor-core
 // kernel with 128-row items, else with 256-row items, which take half the traffic from L2 but keep one of two slots
-// idle where an item has 128 rows or fewer (2048 rows: 345 us against 370 us; 7 to 231 rows: 73 us against 68 us).
-// max_new is a hint, so any choice is right for any lengths.
+// idle where an item has 128 rows or fewer. Eight sequences behind 16384 keys, 4 kv heads of 128, us with 128- / 256-row items:
+// 64 rows 70 / 90, 128 rows 78 / 94, 192 rows 113 / 105, 256 rows 116 / 111, 320 rows 145 / 171, 384 rows 147 / 173,
+// 512 rows 198 / 179, 768 rows 285 / 266, 1024 rows 370 / 340; from 1536 rows on they are within the clock's changes of one
+// another, and behind 1000 to 4000 keys 128-row items are ahead up to 1024 rows (100 / 102). max_new is a hint, so any choice
+// is right for any lengths.
 struct Choice {
   int rows, kt, per_sm;
 };

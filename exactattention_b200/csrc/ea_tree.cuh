@@ -145,10 +145,13 @@ constexpr int MANY_MAX_SEQS = 6000;  // what its shared memory has room for
 int launch_many(const Args& a, bool pair, cudaStream_t st);
 
 // Adds up the partials of the item that share blockIdx.x left unfinished, 16 rows a block (blockIdx.y). It starts
-// while the attention kernel still runs and finds its item meanwhile; after that its cost is the latency of two loads from
-// L2: all of a round's maxima, sums and values are asked for together.
+// while the attention kernel still runs and finds its item meanwhile.
 // Thread (share group, four channels, row): the groups take every G-th share; the groups' sums are joined in a fixed
 // order. A round is COMBINE_SHARES shares; between rounds what has been added up is rescaled to the new maximum.
+// Bound by the latency of loads from L2. A round's maxima and sums are asked for together, of its values COMBINE_AHEAD a
+// thread: all of them where there are four groups or more (64 cells: 2 rows of 128 channels), a quarter with one group (7
+// rows), the rest one after the other. That is what one item over many shares waits for: one token over 16384 keys of one kv head
+// (256 partials, 1.3 us of bytes) takes 61 us a call with 2 rows and 123 us with 8; 131072 keys (296 partials) 84 and 155 us.
 constexpr int COMBINE_THREADS = 256, COMBINE_SHARES = 16, COMBINE_AHEAD = 4;  // values a thread has in flight
 
 template <typename T, int ROWS, int KT, int EXTRA>

@@ -18,12 +18,13 @@
 // Weights are rounded to the cache's type for the product (relative error 2^-9 for bf16; 2^-12 for fp16 down to 2^-25 of the
 // row's largest weight, below that 2^-36 of the largest; of random sign, about the rounding of the output itself);
 // their sum takes them unrounded.
-// Measured on one B200: 16 trees of 17 to 64 nodes over 1K to 15K keys, 16 / 8 heads of 128, 144 us in bursts and 155 us in
+// Measured on one B200: 16 trees of 17 to 64 nodes over 1K to 15K keys, 16 / 8 heads of 128, 140 us in bursts and 155 us in
 // a long loop (545 MB of keys and values: 83 us at the copy rate); four chunks of 256 tokens behind 16K keys, 32 / 4
-// heads, 333 us in bursts and 383 us in a long loop (277 GFLOP: 170 us at
-// the measured bf16 rate; the tensor pipe is active 42% of the time). A slot's cycle at 128 x 128 x 128 is what bounds it:
-// some 1900 cycles for the weights, 400 to store them and hand them over, 1750 for the issue of the 16 products beside
-// busy softmax warps, 400 until the scores are seen, 4800 in all for both slots' tiles.
+// heads, 325 us in bursts and 381 us in a long loop (277 GFLOP: 170 us at
+// the measured bf16 rate; the tensor pipe is active 43% of the time). A slot's cycle at 128 x 128 x 128 is what bounds it. Clock
+// readings in an instrumented copy, whose cycle is 5500 for a tile of either slot: 2000 for the weights, 400 to store them
+// and hand them over, 800 until the issuer is done with the other slot, 1850 for the issue of the 16 products beside busy
+// softmax warps, 400 to 500 until the scores are seen.
 #pragma once
 #include <cuda.h>
 
@@ -43,7 +44,9 @@ constexpr int SLOT_THREADS = 128, LOADERS = 64;
 constexpr int LAUNCH_REGS = 168, SLOT_REGS = 216, OTHER_REGS = 72;
 constexpr uint32_t COL_S = 0, COL_O = 256;  // slot s: + 128 s
 constexpr int PAGE_RING = 16;
-constexpr int EXTRA = 3;  // units for an item's end: some 8000 cycles against 2400 to 2800 of a tile
+// Units for an item's end: some 15000 cycles (instrumented) from its last weights to the next item's first scores, against
+// 5500 of a 256-row item's tile.
+constexpr int EXTRA = 3;
 
 template <int DP, bool PAIR>
 struct Cfg {

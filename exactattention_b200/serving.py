@@ -7,8 +7,9 @@ positions, the draft model's attention over the paged cache, and the logits' pen
   tree_attention  attention of drafted tokens (a tree, a chain, a single token) over the paged cache
   process_logits  penalties for repeated tokens, biases and grammar masks
 
-Ordinary floating-point operators (32-bit arithmetic, outputs rounded once), hand-written CUDA behind
-include/exactattn_serving.h. Drafts are proposals: the bits that count come from the certified
+Ordinary floating-point operators, hand-written CUDA behind include/exactattn_serving.h: 32-bit arithmetic and
+outputs rounded once, except that tree_attention takes its weights into the product with the values as 16-bit
+numbers (a pair of them for up to 16 query rows a kv head, one for more). Drafts are proposals: the bits that count come from the certified
 `cuda.launch`, which verifies them over the same cache. Torch CUDA tensors in and out, asynchronous on
 the current stream, no host synchronisation, capturable in CUDA graphs. There is no CPU path. Nothing is
 recorded for autograd: tensors that require grad are refused (ValueError) unless under torch.no_grad; a
@@ -136,14 +137,17 @@ def tree_attention(q, k_cache, v_cache, page_table, seq_lens, q_start, alpha, *,
     (ea_tree_attention_cuda). q (tokens, q_heads, d) bf16 or fp16, any token and head strides; caches
     (pages, kv_heads, page_size, d), any page, head and row strides; page_table (batch, max_pages),
     seq_lens (batch,) (the step's tokens included), q_start (batch + 1,) int32, as plan_step gives them.
+    Rows of q, of the caches and of `out` (contiguous) start on 16-byte boundaries.
     A token sees its sequence's earlier keys and, of the step's tokens, those whose bit is set in its row
     of tree_mask ((tokens, words) int32, see `tree_mask`); None: itself and the ones before it. Weights are
-    2^(alpha q.k) (formats.default_alpha), as in `cuda.launch`. max_new (the most tokens of any sequence)
-    only tunes tile sizes. Rows past q_start[batch] are not written. Rows of q, of the caches and of `out`
-    (contiguous) start on 16-byte boundaries. Returns out (tokens, q_heads, d), and
-    with return_lse the log2 of the weights' sums (tokens, q_heads) float32; a row that sees no key gives 0
-    and -inf. Values of keys that a row does not see cannot reach it. The result is not certified: it is the
-    draft model's attention, accurate to its type's rounding."""
+    2^(alpha q.k) (formats.default_alpha), as in `cuda.launch`. max_new (the most tokens of any sequence;
+    None: all of q's) picks the kernel and its tiles, and any value is right: pass 1 for single tokens.
+    Rows past q_start[batch] are not written. Returns out (tokens, q_heads, d), and with return_lse the log2
+    of the weights' sums (tokens, q_heads) float32; a row that sees no key gives 0 and -inf. Values of keys
+    that a row does not see cannot reach it. The result is not certified: it is the draft model's attention.
+    For up to 16 query rows a kv head (by max_new) its error is that of the output's rounding; for more,
+    the weights are rounded to the caches' type for the product with the values, and the root mean square
+    error is up to 1.4 times that."""
     r = _native().tree_attention(q, k_cache, v_cache, page_table, seq_lens, q_start, alpha, tree_mask, max_new,
                                  bool(return_lse), out)
     return r if return_lse else r[0]

@@ -6,8 +6,9 @@
  *   ea_tree_attention_cuda  attention of drafted tokens (tree, chain, single token) over a paged cache
  *   ea_process_logits_cuda  penalties for repeated tokens, biases and grammar masks
  *
- * These are ordinary floating-point operators (32-bit arithmetic, outputs rounded once): they
- * serve the draft side of speculative decoding, whose results the certified attention verifies.
+ * These are ordinary floating-point operators: they serve the draft side of speculative decoding,
+ * whose results the certified attention verifies. Arithmetic is 32-bit and outputs are rounded once,
+ * except that the attention's weights enter the product with the values as 16-bit numbers (below).
  * Every pointer is a device pointer, every call is asynchronous on `stream` (a cudaStream_t, NULL =
  * default), allocates nothing, never waits for the host, and may be captured in a CUDA graph.
  * Calls share no state: they may run on several streams at once.
@@ -93,7 +94,10 @@ int ea_rope_cuda(const ea_rope_t* args, void* stream);
  * NULL: j <= i. Key j of sequence b is row j % page_size of page page_table[b][j / page_size].
  * With w_j = 2^(alpha q . k_j) over the visible keys: out = sum w v / sum w, lse = log2 sum w (NULL: not
  * written); a row that sees no key gives 0 and -inf. Head h reads kv head h / (q_heads / kv_heads).
- * What a row does not see cannot reach its output, NaN and infinities included.
+ * What a row does not see cannot reach its output, NaN and infinities included; an infinite value that it
+ * sees with a weight that rounds to zero may give NaN. For up to 16 query rows a kv head (max_new * q_heads /
+ * kv_heads) w enters sum w v as a pair of 16-bit numbers, 2^-17 off or less; for more it is rounded once to
+ * the caches' type (in fp16 to within 2^-36 of the row's largest weight). sum w is 32-bit.
  * bf16 or fp16 (q, caches and out alike), d a multiple of 8 up to 128, rows on 16-byte boundaries (-9
  * otherwise).
  * max_new: the most tokens any sequence has in this step (a hint: it sizes tiles, not results). tokens *
