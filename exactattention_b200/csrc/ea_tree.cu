@@ -12,7 +12,7 @@
 // 16-key slice is 8 KB of K and V at d = 128, for which an SM has about 350 cycles at the measured copy rate, and
 // needs 24 matrix instructions (8 rows; 48 for 16) and 16 ldmatrix of its four sub-partitions.
 // Weights enter P.V as a pair of 16-bit numbers, their rounding and its remainder (relative error 2^-17 for bf16
-// instead of 2^-9; for fp16 2^-22 or 2^-36 of the row's largest weight, whichever is more), which is 8 of those 24
+// instead of 2^-9; for fp16 2^-22 or 2^-35 of the row's largest weight, whichever is more), which is 8 of those 24
 // instructions: the tensor pipe has the room. A row's reference moves seldom (Reference in ea_tree.cuh), so most slices need no
 // reduction over lanes.
 #include "ea_tree.cuh"

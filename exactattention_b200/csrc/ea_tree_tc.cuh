@@ -15,8 +15,8 @@
 // The MMA thread issues PV(t) and then QK of the slot's next tile, so one arrival per cycle tells the slot that its
 // scores are there and that O is at rest: the rescale of O needs no wait of its own. It happens only when a row's
 // reference moves (Reference in ea_tree.cuh; the sum and O share it).
-// Weights are rounded to the cache's type for the product (relative error 2^-9 for bf16; 2^-12 for fp16 down to 2^-25 of the
-// row's largest weight, below that 2^-36 of the largest; of random sign, about the rounding of the output itself);
+// Weights are rounded to the cache's type for the product (relative error 2^-9 for bf16; 2^-12 for fp16 down to 2^-24 of the
+// row's largest weight, below that 2^-35 of the largest; of random sign, about the rounding of the output itself);
 // their sum takes them unrounded.
 // Measured on one B200: 16 trees of 17 to 64 nodes over 1K to 15K keys, 16 / 8 heads of 128, 140 us in bursts and 155 us in
 // a long loop (545 MB of keys and values: 83 us at the copy rate); four chunks of 256 tokens behind 16K keys, 32 / 4

@@ -97,7 +97,7 @@ int ea_rope_cuda(const ea_rope_t* args, void* stream);
  * What a row does not see cannot reach its output, NaN and infinities included; an infinite value that it
  * sees with a weight that rounds to zero may give NaN. For up to 16 query rows a kv head (max_new * q_heads /
  * kv_heads) w enters sum w v as a pair of 16-bit numbers, 2^-17 off or less; for more it is rounded once to
- * the caches' type (in fp16 to within 2^-36 of the row's largest weight). sum w is 32-bit.
+ * the caches' type (in fp16 to within 2^-35 of the row's largest weight). sum w is 32-bit.
  * bf16 or fp16 (q, caches and out alike), d a multiple of 8 up to 128, rows on 16-byte boundaries (-9
  * otherwise).
  * max_new: the most tokens any sequence has in this step (a hint: it sizes tiles, not results). tokens *
